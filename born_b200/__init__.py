@@ -9,6 +9,8 @@ raises.
 """
 from .sampler import (  # noqa: F401
     SamplingConfig,
+    BeamConfig,
+    BeamPool,
     Sampler,
     SamplerError,
     InvalidArgument,

@@ -13,16 +13,23 @@ ERR_UNSUPPORTED = 4
 ERR_NCCL = 5
 ERR_DEVICE_TIMEOUT = 6
 
-ROW_OK, ROW_ALL_MASKED, ROW_NAN, ROW_POS_INF, ROW_OVERFLOW, ROW_BAD_TOKEN, ROW_FINISHED, ROW_BAD_PARAMS = range(8)
+(ROW_OK, ROW_ALL_MASKED, ROW_NAN, ROW_POS_INF, ROW_OVERFLOW, ROW_BAD_TOKEN, ROW_FINISHED, ROW_BAD_PARAMS,
+ ROW_DEAD) = range(9)
 
 MAX_TOP_K = 1024
 MAX_HISTORY = 1024
 MAX_DRAFT = 16
 MAX_SHARDS = 16
+MAX_BEAMS = 16
+MAX_STOPS = 8
+MAX_REORDER = 128
+MAX_STEPS = 16384
 DTYPE_F32, DTYPE_BF16 = 0, 1
 MEM_DEVICE, MEM_HOST = 0, 1
 FLAG_GREEDY = 1
 FLAG_FULL_VOCAB = 2
+BEAM_KEEP_SLOTS = 1
+BEAM_EARLY_STOP = 2
 
 
 class RowParams(C.Structure):
@@ -111,6 +118,84 @@ class ShardArgs(C.Structure):
     ]
 
 
+class BeamArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("memory", C.c_uint32),
+        ("groups", C.c_int32),
+        ("beams", C.c_int32),
+        ("vocab", C.c_int32),
+        ("logits_dtype", C.c_int32),
+        ("logits_row_stride", C.c_int64),
+        ("logits", C.c_void_p),
+        ("mask", C.c_void_p),
+        ("mask_row_stride", C.c_int64),
+        ("history", C.c_void_p),
+        ("history_len", C.c_void_p),
+        ("history_stride", C.c_int32),
+        ("flags", C.c_uint32),
+        ("params", RowParams),
+        ("scores", C.c_void_p),
+        ("stop_ids", C.c_int32 * MAX_STOPS),
+        ("n_stop", C.c_int32),
+        ("step", C.c_int32),
+        ("out_parent", C.c_void_p),
+        ("out_token", C.c_void_p),
+        ("out_score", C.c_void_p),
+        ("out_status", C.c_void_p),
+        ("out_end_parent", C.c_void_p),
+        ("out_end_token", C.c_void_p),
+        ("out_end_score", C.c_void_p),
+        ("pool_score", C.c_void_p),
+        ("pool_step", C.c_void_p),
+        ("pool_parent", C.c_void_p),
+        ("pool_token", C.c_void_p),
+        ("done", C.c_void_p),
+        ("length_penalty", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
+class ReorderArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("memory", C.c_uint32),
+        ("groups", C.c_int32),
+        ("beams", C.c_int32),
+        ("n_buffers", C.c_int32),
+        ("planes", C.c_int32),
+        ("buffers", C.POINTER(C.c_void_p)),
+        ("row_stride", C.c_int64),
+        ("plane_stride", C.c_int64),
+        ("position_bytes", C.c_int64),
+        ("positions", C.c_int64),
+        ("parents", C.c_void_p),
+        ("lens", C.c_void_p),
+    ]
+
+
+class SequencesArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("memory", C.c_uint32),
+        ("groups", C.c_int32),
+        ("beams", C.c_int32),
+        ("steps", C.c_int32),
+        ("hypotheses", C.c_int32),
+        ("table_stride", C.c_int64),
+        ("tokens", C.c_void_p),
+        ("parents", C.c_void_p),
+        ("end_step", C.c_void_p),
+        ("end_parent", C.c_void_p),
+        ("end_token", C.c_void_p),
+        ("out_tokens", C.c_void_p),
+        ("out_stride", C.c_int64),
+        ("out_lens", C.c_void_p),
+        ("pad", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/born_sampler.h
 SYMBOLS = {
     "born_sampler_create": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
@@ -130,6 +215,11 @@ SYMBOLS = {
     "born_mask_commit": (C.c_int32, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "born_mask_wait": (C.c_int32, [C.c_void_p, C.c_void_p]),
     "born_spec_verify": (C.c_int32, [C.c_void_p, C.POINTER(SpecArgs), C.c_void_p]),
+    "born_beam_step": (C.c_int32, [C.c_void_p, C.POINTER(BeamArgs), C.c_void_p]),
+    "born_beam_next": (C.c_int32, [C.c_void_p, C.POINTER(BeamArgs), C.c_void_p]),
+    "born_beam_pool_reset": (C.c_int32, [C.c_void_p, C.POINTER(BeamArgs), C.c_void_p]),
+    "born_beam_reorder": (C.c_int32, [C.c_void_p, C.POINTER(ReorderArgs), C.c_void_p]),
+    "born_beam_sequences": (C.c_int32, [C.c_void_p, C.POINTER(SequencesArgs), C.c_void_p]),
     "born_shard_record_bytes": (C.c_int32, [C.c_int32]),
     "born_shard_unique_id": (C.c_int32, [C.c_void_p]),
     "born_shard_init": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32]),

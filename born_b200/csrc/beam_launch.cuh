@@ -1,0 +1,84 @@
+// Host-side entry points of the beam-search kernels, instantiated in beam.cu.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include "../../include/born_sampler.h"
+
+namespace born {
+
+constexpr int kBeamMaxSlices = 64;    // slices of a row: two records per lane of the warp that merges them
+
+// What a slice leaves for the merge.
+struct BeamRecord {
+    double sum;  // sum exp((z - max)/T) over the slice
+    float max;   // NaN / +inf: the slice holds one
+    uint32_t pad;
+    float stop_z[BORN_MAX_STOPS];  // penalised logits of the stop tokens in the slice, -inf elsewhere
+    unsigned long long list[BORN_MAX_BEAMS];  // rank keys of the best tokens, 0 = none
+};
+
+struct BeamArgs {
+    int N, K, V, slices;
+    const void* logits;
+    int64_t row_stride;
+    const uint32_t* mask;
+    int64_t mask_stride;
+    const int32_t* history;
+    const int32_t* history_len;
+    int history_stride;
+    uint32_t flags;
+    born_row_params params;
+    float temperature, scale_log2e;  // T; log2(e)/T
+    double slack;   // two normalisers in 32 bits are off by less than this together
+    int bit_words;  // words of a CTA's bit map
+    const float* scores;
+    int32_t stop_ids[BORN_MAX_STOPS];
+    int n_stop, step;
+    int32_t *out_parent, *out_token;
+    float* out_score;
+    int32_t* out_status;
+    int32_t *out_end_parent, *out_end_token;
+    float* out_end_score;
+    float* pool_score;
+    int32_t *pool_step, *pool_parent, *pool_token, *done;
+    double length_norm;
+    // workspace
+    BeamRecord* records;
+    uint32_t* tickets;
+    // device-resident history (born_beam_next)
+    int32_t *ring, *ring_total, *ring_len;
+    int ring_cap;
+};
+
+// Slices per row for a launch of `rows` rows.
+int beam_slices(int rows, int vocab, int num_sms);
+// Records that launches of up to max_batch rows of up to max_vocab tokens leave.
+int64_t beam_max_records(int max_batch, int max_vocab, int num_sms);
+cudaError_t beam_attrs();
+cudaError_t beam_launch(BeamArgs& A, int dtype, cudaStream_t st);
+
+// ---- born_beam_reorder ------------------------------------------------------------------------
+struct ReorderArgs {
+    int N, K, n_buffers, planes;
+    int64_t row_stride, plane_stride, position_bytes, positions;
+    int64_t chunk;   // bytes of a piece that a CTA moves
+    int chunks;      // of a piece
+    const int32_t* parents;
+    const int32_t* lens;
+    uint8_t* buffers[BORN_MAX_REORDER];
+};
+cudaError_t reorder_launch(ReorderArgs& A, cudaStream_t st);
+
+// ---- born_beam_sequences ------------------------------------------------------------------------
+constexpr int kSequenceMaxSteps = 16384;  // the steps' maps fill 160 KB of shared memory
+struct SequencesArgs {
+    int N, K, T, H;
+    int64_t table_stride, out_stride;
+    const int32_t *tokens, *parents, *end_step, *end_parent, *end_token;
+    int32_t *out_tokens, *out_lens;
+    int32_t pad;
+};
+cudaError_t sequences_attrs();
+cudaError_t sequences_launch(const SequencesArgs& A, cudaStream_t st);
+
+}  // namespace born

@@ -19,6 +19,7 @@
 #include "merge_kernel.cuh"
 #include "prepass.cuh"
 #include "spec_kernel.cuh"
+#include "beam_launch.cuh"
 
 using namespace born;
 
@@ -71,6 +72,10 @@ struct Handle {
     int n_stop = 0;
     int32_t stop_ids[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     bool use_ring = false;         // set by born_sample_next around its call of sample_device
+    // beam search: the slices' records and a ticket per group
+    BeamRecord* beam_records = nullptr;
+    int64_t beam_records_cap = 0;
+    uint32_t* beam_tickets = nullptr;
     // grammar-mask upload (born_mask_*)
     uint32_t* mask_host[2] = {nullptr, nullptr};
     uint32_t* mask_dev[2] = {nullptr, nullptr};
@@ -421,11 +426,16 @@ int32_t born_sampler_create(int32_t device, int32_t max_batch, int32_t max_vocab
     if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->tickets, sp.tickets);
     if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->seg_packed, sp.seg_packed);
     if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->dev_error, 32 * sizeof(int));
+    h->beam_records_cap = beam_max_records(max_batch, max_vocab, h->num_sms);
+    if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->beam_records, (size_t)h->beam_records_cap * sizeof(BeamRecord));
+    if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->beam_tickets, sizeof(uint32_t) * (size_t)max_batch);
+    if (rc == BORN_OK && cudaMemset(h->beam_tickets, 0, sizeof(uint32_t) * (size_t)max_batch) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cudaMemset(h->tickets, 0, sp.tickets) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cudaMemset(h->dev_error, 0, 32 * sizeof(int)) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && scan_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cluster_limits(h->max_clusters) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && spec_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
+    if (rc == BORN_OK && (beam_attrs() != cudaSuccess || sequences_attrs() != cudaSuccess)) rc = BORN_ERR_CUDA;
     for (int i = 0; i < 4 && rc == BORN_OK; ++i)
         if (cudaEventCreate(&h->ev[i]) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc != BORN_OK) {
@@ -455,6 +465,8 @@ int32_t born_sampler_destroy(void* handle) {
     cudaFree(h->tickets);
     cudaFree(h->seg_packed);
     cudaFree(h->dev_error);
+    cudaFree(h->beam_records);
+    cudaFree(h->beam_tickets);
     cudaFree(h->spec_scratch);
     cudaFree(h->clean_copy);
     cudaFree(h->gathered);
@@ -1043,6 +1055,220 @@ int32_t born_debug_mass(const float* x, uint64_t* q, int64_t n, void* stream) {
     if (n == 0) return BORN_OK;
     debug_mass_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (cudaStream_t)stream>>>(x, (unsigned long long*)q, n);
     return cudaGetLastError() == cudaSuccess ? BORN_OK : BORN_ERR_CUDA;
+}
+
+// ------------------------------------------------------------------ beam search
+}  // extern "C"
+namespace {
+// The handle's device for the length of a call; the caller's current device afterwards.
+struct DeviceScope {
+    int before = -1;
+    int rc;
+    explicit DeviceScope(Handle* h) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        rc = use_device(h);
+        if (before == h->device) before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+template <typename Args>
+int args_check(Handle* h, const Args* a, const char* what) {
+    if (!a) return fail(h, BORN_ERR_INVALID_ARGUMENT, "%s: args is NULL", what);
+    if (a->struct_size != sizeof(Args)) return fail(h, BORN_ERR_INVALID_ARGUMENT, "%s: struct_size %u != %zu", what, a->struct_size, sizeof(Args));
+    if (a->memory != BORN_MEM_DEVICE)
+        return fail(h, a->memory == BORN_MEM_HOST ? BORN_ERR_UNSUPPORTED : BORN_ERR_INVALID_ARGUMENT, "%s takes device memory", what);
+    if (h->is_static) return fail(h, BORN_ERR_UNSUPPORTED, "%s needs a handle", what);
+    return BORN_OK;
+}
+int groups_check(Handle* h, int groups, int beams, const char* what) {
+    if (groups < 1 || beams < 1) return fail(h, BORN_ERR_INVALID_ARGUMENT, "%s: groups %d and beams %d must be positive", what, groups, beams);
+    if (beams > BORN_MAX_BEAMS) return fail(h, BORN_ERR_UNSUPPORTED, "%s: %d beams exceed %d", what, beams, BORN_MAX_BEAMS);
+    return BORN_OK;
+}
+bool unaligned(const void* p, size_t to) { return (uintptr_t)p % to != 0; }
+
+int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
+    int rc = args_check(h, a, "beam_step");
+    if (rc || (rc = groups_check(h, a->groups, a->beams, "beam_step"))) return rc;
+    const int64_t rows = (int64_t)a->groups * a->beams;
+    if (a->vocab <= 0) return fail(h, BORN_ERR_INVALID_ARGUMENT, "vocab must be positive");
+    if (rows > h->max_batch || a->vocab > h->max_vocab)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "%lld rows / vocab %d exceed the handle's %d / %d", (long long)rows, a->vocab, h->max_batch, h->max_vocab);
+    if (a->logits_dtype != BORN_DTYPE_F32 && a->logits_dtype != BORN_DTYPE_BF16)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "unknown logits_dtype %d", a->logits_dtype);
+    if (!a->logits || !a->scores || !a->out_parent || !a->out_token || !a->out_score)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "logits, scores, out_parent, out_token and out_score are required");
+    if (a->logits_row_stride < a->vocab) return fail(h, BORN_ERR_INVALID_ARGUMENT, "logits_row_stride < vocab");
+    if (unaligned(a->logits, a->logits_dtype == BORN_DTYPE_F32 ? 4 : 2)) return fail(h, BORN_ERR_INVALID_ARGUMENT, "logits pointer is not aligned to its element size");
+    if (a->mask && (a->mask_row_stride < (a->vocab + 31) / 32 || unaligned(a->mask, 4)))
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "mask_row_stride < ceil(vocab/32), or mask is not 4-byte aligned");
+    if (a->history && (a->history_stride <= 0 || a->history_stride > BORN_MAX_HISTORY))
+        return fail(h, a->history_stride > BORN_MAX_HISTORY ? BORN_ERR_UNSUPPORTED : BORN_ERR_INVALID_ARGUMENT,
+                    "history_stride %d outside 1..%d", a->history_stride, BORN_MAX_HISTORY);
+    if (!params_ok(a->params)) return fail(h, BORN_ERR_INVALID_ARGUMENT, "temperature or penalties out of range");
+    if (a->params.top_k || a->params.top_p != 0.0f || a->params.min_p != 0.0f || a->params.flags)
+        return fail(h, BORN_ERR_UNSUPPORTED, "beam search takes a temperature and penalties, no top_k, top_p, min_p or flags");
+    if (a->flags & ~(BORN_BEAM_KEEP_SLOTS | BORN_BEAM_EARLY_STOP)) return fail(h, BORN_ERR_INVALID_ARGUMENT, "unknown beam flags 0x%x", a->flags);
+    if (a->n_stop < 0 || a->n_stop > BORN_MAX_STOPS) return fail(h, BORN_ERR_INVALID_ARGUMENT, "0..%d stop tokens", BORN_MAX_STOPS);
+    if (!a->out_end_parent != !a->out_end_token || !a->out_end_parent != !a->out_end_score)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "out_end_parent, out_end_token and out_end_score go together");
+    if (!a->pool_score != !a->pool_step || !a->pool_score != !a->pool_parent || !a->pool_score != !a->pool_token || !a->pool_score != !a->done)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "the pool's five arrays go together");
+    if (a->pool_score && (a->step < 0 || !isfinite(a->length_penalty))) return fail(h, BORN_ERR_INVALID_ARGUMENT, "step %d or length_penalty out of range", a->step);
+    DeviceScope on(h);
+    if (on.rc) return on.rc;
+    BeamArgs A;
+    memset(&A, 0, sizeof A);
+    A.N = a->groups; A.K = a->beams; A.V = a->vocab;
+    A.slices = beam_slices((int)rows, a->vocab, h->num_sms);
+    if (rows * A.slices > h->beam_records_cap) return fail(h, BORN_ERR_UNSUPPORTED, "batch x vocab exceeds the workspace");
+    A.logits = a->logits; A.row_stride = a->logits_row_stride;
+    A.mask = a->mask; A.mask_stride = a->mask_row_stride;
+    A.params = a->params;
+    if (host_penalties_on(a->params)) {
+        A.history = a->history; A.history_len = a->history_len; A.history_stride = a->history_stride;
+    }
+    A.flags = a->flags;
+    A.temperature = a->params.temperature == 0.0f ? 1.0f : a->params.temperature;
+    A.scale_log2e = (float)(M_LOG2E / (double)A.temperature);
+    A.scores = a->scores;
+    for (int i = 0; i < a->n_stop; ++i) {  // those of the vocabulary, each once
+        const int32_t t = a->stop_ids[i];
+        bool known = t < 0 || t >= a->vocab;
+        for (int j = 0; j < A.n_stop; ++j) known = known || A.stop_ids[j] == t;
+        if (!known) A.stop_ids[A.n_stop++] = t;
+    }
+    A.step = a->step;
+    A.out_parent = a->out_parent; A.out_token = a->out_token; A.out_score = a->out_score; A.out_status = a->out_status;
+    A.out_end_parent = a->out_end_parent; A.out_end_token = a->out_end_token; A.out_end_score = a->out_end_score;
+    A.pool_score = a->pool_score; A.pool_step = a->pool_step; A.pool_parent = a->pool_parent; A.pool_token = a->pool_token;
+    A.done = a->done;
+    A.length_norm = pow((double)a->step + 1.0, (double)a->length_penalty);
+    A.records = h->beam_records;
+    A.tickets = h->beam_tickets;
+    if (ring) {
+        A.ring = h->ring;
+        A.ring_total = h->ring + (size_t)h->max_batch * h->ring_cap;
+        A.ring_len = A.ring_total + h->max_batch;
+        A.ring_cap = h->ring_cap;
+    }
+    CUDA_TRY(h, beam_launch(A, a->logits_dtype, st));
+    h->launches++;
+    return BORN_OK;
+}
+
+__global__ void pool_reset_kernel(float* score, int32_t* step, int32_t* parent, int32_t* token, int32_t* done, int n, int groups) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) {
+        score[i] = -INFINITY;
+        step[i] = parent[i] = token[i] = -1;
+    }
+    if (i < groups) done[i] = 0;
+}
+}  // namespace
+extern "C" {
+
+int32_t born_beam_step(void* handle, const born_beam_args* a, void* stream) {
+    Handle* h = (Handle*)handle;
+    if (!h) return fail(nullptr, BORN_ERR_INVALID_ARGUMENT, "handle is NULL");
+    return beam_run(h, a, false, (cudaStream_t)stream);
+}
+
+int32_t born_beam_next(void* handle, const born_beam_args* a, void* stream) {
+    Handle* h = (Handle*)handle;
+    if (!h) return fail(nullptr, BORN_ERR_INVALID_ARGUMENT, "handle is NULL");
+    if (!h->ring) return fail(h, BORN_ERR_INVALID_ARGUMENT, "born_history_create has not been called");
+    const int rc = args_check(h, a, "beam_next");
+    if (rc) return rc;
+    if (a->history || a->history_len) return fail(h, BORN_ERR_INVALID_ARGUMENT, "born_beam_next reads the handle's history: args->history must be NULL");
+    born_beam_args d = *a;
+    d.history = h->ring;
+    d.history_len = h->ring + (size_t)h->max_batch * h->ring_cap + h->max_batch;
+    d.history_stride = h->ring_cap;
+    return beam_run(h, &d, true, (cudaStream_t)stream);
+}
+
+int32_t born_beam_pool_reset(void* handle, const born_beam_args* a, void* stream) {
+    Handle* h = (Handle*)handle;
+    if (!h) return fail(nullptr, BORN_ERR_INVALID_ARGUMENT, "handle is NULL");
+    int rc = args_check(h, a, "beam_pool_reset");
+    if (rc || (rc = groups_check(h, a->groups, a->beams, "beam_pool_reset"))) return rc;
+    if (!a->pool_score || !a->pool_step || !a->pool_parent || !a->pool_token || !a->done)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "the pool's five arrays are required");
+    if ((int64_t)a->groups * a->beams > h->max_batch) return fail(h, BORN_ERR_INVALID_ARGUMENT, "groups x beams exceed the handle's %d rows", h->max_batch);
+    DeviceScope on(h);
+    if (on.rc) return on.rc;
+    const int n = a->groups * a->beams;
+    pool_reset_kernel<<<(n + 255) / 256, 256, 0, (cudaStream_t)stream>>>(a->pool_score, a->pool_step, a->pool_parent, a->pool_token, a->done, n, a->groups);
+    CUDA_TRY(h, cudaGetLastError());
+    h->launches++;
+    return BORN_OK;
+}
+
+int32_t born_beam_reorder(void* handle, const born_reorder_args* a, void* stream) {
+    Handle* h = (Handle*)handle;
+    if (!h) return fail(nullptr, BORN_ERR_INVALID_ARGUMENT, "handle is NULL");
+    int rc = args_check(h, a, "beam_reorder");
+    if (rc || (rc = groups_check(h, a->groups, a->beams, "beam_reorder"))) return rc;
+    if (a->n_buffers < 1 || a->planes < 1 || a->position_bytes < 1 || a->positions < 0 || !a->buffers || !a->parents)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: buffers, parents, planes and position_bytes are required");
+    if (a->n_buffers > BORN_MAX_REORDER) return fail(h, BORN_ERR_UNSUPPORTED, "beam_reorder: %d buffers exceed %d", a->n_buffers, BORN_MAX_REORDER);
+    if (a->positions > INT64_MAX / 8 / a->position_bytes) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: positions x position_bytes out of range");
+    const int64_t piece = a->positions * a->position_bytes;
+    const bool one_row = (int64_t)a->groups * a->beams == 1;
+    // the pieces of a row lie apart, and the rows; in either order
+    bool apart;
+    if (a->row_stride >= a->plane_stride || a->planes == 1)
+        apart = (a->planes == 1 || a->plane_stride >= piece) && (one_row || a->row_stride >= (a->planes - 1) * (a->planes > 1 ? a->plane_stride : 0) + piece);
+    else
+        apart = a->row_stride >= piece && a->plane_stride >= ((int64_t)a->groups * a->beams - 1) * a->row_stride + piece;
+    if (!apart) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: rows or pieces overlap (row_stride %lld, plane_stride %lld, piece %lld bytes)",
+                            (long long)a->row_stride, (long long)a->plane_stride, (long long)piece);
+    if ((int64_t)a->groups * a->n_buffers * a->planes > 0x7fffffff / 4) return fail(h, BORN_ERR_UNSUPPORTED, "beam_reorder: too many pieces for one call");
+    ReorderArgs A;
+    memset(&A, 0, sizeof A);
+    for (int i = 0; i < a->n_buffers; ++i) {
+        if (!a->buffers[i]) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: buffer %d is NULL", i);
+        A.buffers[i] = (uint8_t*)a->buffers[i];
+    }
+    if (a->beams == 1) return BORN_OK;
+    DeviceScope on(h);
+    if (on.rc) return on.rc;
+    A.N = a->groups; A.K = a->beams; A.n_buffers = a->n_buffers; A.planes = a->planes;
+    A.row_stride = a->row_stride; A.plane_stride = a->plane_stride;
+    A.position_bytes = a->position_bytes; A.positions = a->positions;
+    A.parents = a->parents; A.lens = a->lens;
+    CUDA_TRY(h, reorder_launch(A, (cudaStream_t)stream));
+    h->launches++;
+    return BORN_OK;
+}
+
+int32_t born_beam_sequences(void* handle, const born_sequences_args* a, void* stream) {
+    Handle* h = (Handle*)handle;
+    if (!h) return fail(nullptr, BORN_ERR_INVALID_ARGUMENT, "handle is NULL");
+    int rc = args_check(h, a, "beam_sequences");
+    if (rc || (rc = groups_check(h, a->groups, a->beams, "beam_sequences"))) return rc;
+    if (a->steps < 1 || a->hypotheses < 1) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_sequences: steps and hypotheses must be positive");
+    if (a->steps > BORN_MAX_STEPS || a->hypotheses > BORN_MAX_BEAMS)
+        return fail(h, BORN_ERR_UNSUPPORTED, "beam_sequences: %d steps / %d hypotheses exceed %d / %d", a->steps, a->hypotheses, BORN_MAX_STEPS, BORN_MAX_BEAMS);
+    if (a->table_stride < (int64_t)a->groups * a->beams || a->out_stride < a->steps)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_sequences: table_stride < groups x beams, or out_stride < steps");
+    if (!a->tokens || !a->parents || !a->end_step || !a->end_parent || !a->end_token || !a->out_tokens || !a->out_lens)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_sequences: a required pointer is NULL");
+    DeviceScope on(h);
+    if (on.rc) return on.rc;
+    SequencesArgs A;
+    A.N = a->groups; A.K = a->beams; A.T = a->steps; A.H = a->hypotheses;
+    A.table_stride = a->table_stride; A.out_stride = a->out_stride;
+    A.tokens = a->tokens; A.parents = a->parents;
+    A.end_step = a->end_step; A.end_parent = a->end_parent; A.end_token = a->end_token;
+    A.out_tokens = a->out_tokens; A.out_lens = a->out_lens; A.pad = a->pad;
+    CUDA_TRY(h, sequences_launch(A, (cudaStream_t)stream));
+    h->launches++;
+    return BORN_OK;
 }
 
 // ------------------------------------------------------------------ speculative verify

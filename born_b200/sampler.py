@@ -70,6 +70,38 @@ class SamplingConfig:
                            self.frequency_penalty, self.presence_penalty, self.flags())
 
 
+@dataclass
+class BeamConfig:
+    """A step of beam search.  Zero values mean "off"; temperature 0 means 1."""
+    temperature: float = 0.0
+    repetition_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    stop_tokens: tuple = ()
+    length_penalty: float = 0.0  # pooled hypotheses are compared by score / length ** length_penalty
+    early_stop: bool = False     # a group is done as soon as its pool is full
+    keep_slots: bool = False     # the best child of a beam stays in the beam's row: fewer states move
+
+    def flags(self):
+        return (L.BEAM_KEEP_SLOTS if self.keep_slots else 0) | (L.BEAM_EARLY_STOP if self.early_stop else 0)
+
+
+class BeamPool:
+    """The best ended hypotheses of every group, on the device (see `Sampler.beam_pool`).
+
+    score [groups, beams] fp32 (normalised, -inf = free), step / parent / token [groups, beams] int32,
+    done [groups] int32."""
+
+    def __init__(self, groups, beams, device):
+        self.score = torch.empty((groups, beams), dtype=torch.float32, device=device)
+        self.step, self.parent, self.token = (torch.empty((groups, beams), dtype=torch.int32, device=device) for _ in range(3))
+        self.done = torch.empty((groups,), dtype=torch.int32, device=device)
+
+    def into(self, a):
+        a.pool_score, a.pool_step, a.pool_parent, a.pool_token, a.done = (
+            x.data_ptr() for x in (self.score, self.step, self.parent, self.token, self.done))
+
+
 ROW_PARAMS_DTYPE = np.dtype([
     ("temperature", "<f4"), ("top_p", "<f4"), ("min_p", "<f4"), ("top_k", "<i4"),
     ("repetition_penalty", "<f4"), ("frequency_penalty", "<f4"), ("presence_penalty", "<f4"), ("flags", "<u4"),
@@ -126,17 +158,18 @@ def _logits_dtype(x, bf16_hint):
 
 
 class PreparedCall:
-    """A marshalled `born_sample` call (see `Sampler.prepare`)."""
+    """A marshalled call (see `Sampler.prepare` and the `prepare_*` methods)."""
 
-    def __init__(self, sampler, out):
+    def __init__(self, sampler, out, fn=None, args=None, keep=None):
         self._s = sampler
-        self._fn = sampler._lib.born_sample
-        self.args = None
+        self._fn = fn or sampler._lib.born_sample
+        self.args = args
         self.out = out
+        self._keep = keep  # the buffers that the arguments point to
 
     def set_logits(self, logits):
         self.args.logits = _ptr(logits)
-        self._keep = logits
+        self._logits = logits
 
     def run(self, stream=None):
         rc = self._fn(self._s._h, C.byref(self.args), stream)
@@ -416,6 +449,214 @@ class Sampler:
         if rc != L.BORN_OK:
             self._raise(rc)
         return res
+
+    # -- beam search ------------------------------------------------------------------------
+    def _device_tensor(self, name, x, dtype=None, numel=None, contiguous=True):
+        """Check a required device tensor; returns its pointer."""
+        if not _on_device(x):
+            raise InvalidArgument(f"{name} must be a CUDA tensor")
+        if x.device.index != self.device:
+            raise InvalidArgument(f"{name} is on {x.device}, the sampler on cuda:{self.device}")
+        if dtype is not None and x.dtype != dtype:
+            raise InvalidArgument(f"{name} must be {dtype}, not {x.dtype}")
+        if numel is not None and x.numel() != numel:
+            raise InvalidArgument(f"{name} must have {numel} elements, not {x.numel()}")
+        if contiguous:
+            _check_contig(name, x)
+        return x.data_ptr()
+
+    def beam_pool(self, groups, beams, stream=None):
+        """An empty pool for the hypotheses that end."""
+        pool = BeamPool(int(groups), int(beams), f"cuda:{self.device}")
+        self.beam_pool_reset(pool, stream=stream)
+        return pool
+
+    def beam_pool_reset(self, pool, stream=None):
+        """Empty a pool for the next search."""
+        a = L.BeamArgs()
+        a.struct_size, a.memory = C.sizeof(L.BeamArgs), L.MEM_DEVICE
+        a.groups, a.beams = (int(n) for n in pool.score.shape)
+        pool.into(a)
+        rc = self._lib.born_beam_pool_reset(self._h, C.byref(a), stream)
+        if rc != L.BORN_OK:
+            self._raise(rc)
+
+    def prepare_beam_step(self, logits, scores, beams, config=None, mask=None, history=None, history_len=None, pool=None,
+                          step=0, out=None, device_history=False):
+        """Marshal a `beam_step` (with device_history: a `beam_next`) call once; `run(stream)` then costs one
+        foreign call.  The buffers must stay in place; `args.step` may be set between runs."""
+        if not _on_device(logits) or logits.ndim != 2:
+            raise InvalidArgument("beam_step: logits must be a 2D CUDA tensor [groups * beams, vocab]")
+        self._device_tensor("logits", logits, contiguous=False)
+        R, V = int(logits.shape[0]), int(logits.shape[1])
+        beams = int(beams)
+        if beams < 1 or R % beams:
+            raise InvalidArgument(f"{R} rows are not a multiple of {beams} beams")
+        if logits.stride(1) != 1 and V > 1:
+            raise InvalidArgument("logits rows must be contiguous")
+        c = config or BeamConfig()
+        a = L.BeamArgs()
+        a.struct_size, a.memory = C.sizeof(L.BeamArgs), L.MEM_DEVICE
+        a.groups, a.beams, a.vocab = R // beams, beams, V
+        a.logits_dtype = _logits_dtype(logits, False)
+        a.logits_row_stride = int(logits.stride(0)) if R > 1 else V
+        a.logits = logits.data_ptr()
+        if mask is not None:
+            if mask.ndim != 2 or int(mask.shape[0]) != R or mask.element_size() != 4:
+                raise InvalidArgument("mask must be [groups * beams, ceil(vocab/32)] 32-bit words")
+            a.mask, a.mask_row_stride = self._device_tensor("mask", mask), int(mask.shape[1])
+        if history is not None:
+            if history.ndim != 2 or int(history.shape[0]) != R:
+                raise InvalidArgument("history must be [groups * beams, n] int32")
+            if int(history.shape[1]) > 0:
+                a.history, a.history_stride = self._device_tensor("history", history, torch.int32), int(history.shape[1])
+                if history_len is not None:
+                    a.history_len = self._device_tensor("history_len", history_len, torch.int32, R)
+        elif history_len is not None:
+            raise InvalidArgument("history_len without history")
+        a.params = L.RowParams(c.temperature, 0.0, 0.0, 0, c.repetition_penalty, c.frequency_penalty, c.presence_penalty, 0)
+        a.flags, a.length_penalty, a.step = c.flags(), c.length_penalty, int(step)
+        if len(c.stop_tokens) > L.MAX_STOPS:
+            raise InvalidArgument(f"at most {L.MAX_STOPS} stop tokens")
+        a.n_stop = len(c.stop_tokens)
+        for i, t in enumerate(c.stop_tokens):
+            a.stop_ids[i] = int(t)
+        a.scores = self._device_tensor("scores", scores, torch.float32, R)
+        if pool is not None:
+            if tuple(pool.score.shape) != (R // beams, beams):
+                raise InvalidArgument(f"pool is {tuple(pool.score.shape)}, not {(R // beams, beams)}")
+            self._device_tensor("pool", pool.score)
+            pool.into(a)
+        res = out if out is not None else {}
+        dev = logits.device
+        i32, f32 = torch.int32, torch.float32
+        names = [("parent", i32), ("token", i32), ("score", f32), ("status", i32)]
+        ends = [("end_parent", i32), ("end_token", i32), ("end_score", f32)] if a.n_stop else []
+        for name, dtype in names + ends:
+            if name not in res:
+                res[name] = torch.empty((R // beams, beams) if name.startswith("end_") else (R,), dtype=dtype, device=dev)
+            setattr(a, "out_" + name, self._device_tensor("out " + name, res[name], dtype, R))
+        fn = self._lib.born_beam_next if device_history else self._lib.born_beam_step
+        if device_history and (history is not None or history_len is not None):
+            raise InvalidArgument("beam_next reads the sampler's own history")
+        return PreparedCall(self, res, fn, a, (logits, scores, mask, history, history_len, pool))
+
+    def beam_step(self, logits, scores, beams, stream=None, **kw):
+        """One step of beam search over logits [groups * beams, vocab] and the beams' log-probabilities
+        `scores` [groups * beams] (-inf: no such beam, as all but the first of a group before its first step).
+
+        Returns parent (beam of the same group), token (-1: none) and score of the beams that go on and
+        the status of the rows, each [groups * beams]; with stop tokens also end_parent / end_token /
+        end_score [groups, beams] of the hypotheses that end in this step, best first, padded with -1 and
+        -inf.  With `pool` (from `beam_pool`) they join it and groups that are done are passed over."""
+        return self.prepare_beam_step(logits, scores, beams, **kw).run(stream)
+
+    def beam_next(self, logits, scores, beams, stream=None, **kw):
+        """`beam_step` over the device-resident history, a row per beam: the kernel moves the histories after
+        the beams and appends their tokens."""
+        return self.prepare_beam_step(logits, scores, beams, device_history=True, **kw).run(stream)
+
+    def prepare_beam_reorder(self, states, parents, beams, lens=None, position_dim=None):
+        """Marshal a `beam_reorder` call once."""
+        states = list(states)
+        if not states:
+            raise InvalidArgument("beam_reorder: no states")
+        first = states[0]
+        for i, x in enumerate(states):
+            self._device_tensor(f"states[{i}]", x, contiguous=False)
+            if x.shape != first.shape or x.stride() != first.stride() or x.dtype != first.dtype:
+                raise InvalidArgument("beam_reorder: the states of one call have one shape, stride and dtype")
+        if first.ndim < 1:
+            raise InvalidArgument("beam_reorder: states are [groups * beams, ...]")
+        R, beams = int(first.shape[0]), int(beams)
+        if beams < 1 or R % beams or R == 0:
+            raise InvalidArgument(f"{R} rows are not a multiple of {beams} beams")
+        if lens is not None and position_dim is None:
+            raise InvalidArgument("beam_reorder: lens needs position_dim")
+        dims = [(int(n), int(s)) for n, s in zip(first.shape, first.stride())][1:]
+        at = len(dims) if position_dim is None else int(position_dim) - 1
+        if position_dim is not None and not 0 <= at < len(dims):
+            raise InvalidArgument(f"position_dim {position_dim} outside 1..{first.ndim - 1}")
+        # behind the positions: one contiguous block
+        width = 1
+        for n, s in reversed(dims[at + 1:]):
+            if n != 1 and s != width:
+                raise InvalidArgument("beam_reorder: what lies behind the positions must be contiguous")
+            width *= n
+        if position_dim is None:
+            positions, front = 1, dims
+        else:
+            positions, front = dims[at][0], dims[:at]
+            if positions > 1 and dims[at][1] != width:
+                raise InvalidArgument("beam_reorder: positions must be contiguous")
+        # in front of them: pieces at one stride, where they do not continue the block
+        planes, plane_stride = 1, 0
+        for n, s in reversed(front):
+            if n == 1:
+                continue
+            if planes == 1 and position_dim is None and s == width:
+                width *= n
+            elif planes == 1:
+                planes, plane_stride = n, s
+            elif s == planes * plane_stride:
+                planes *= n
+            else:
+                raise InvalidArgument("beam_reorder: the dimensions in front of the positions must have one stride")
+        if first.numel() == 0:
+            raise InvalidArgument("beam_reorder: empty states")
+        esz = first.element_size()
+        a = L.ReorderArgs()
+        a.struct_size, a.memory = C.sizeof(L.ReorderArgs), L.MEM_DEVICE
+        a.groups, a.beams, a.n_buffers, a.planes = R // beams, beams, len(states), planes
+        pointers = (C.c_void_p * len(states))(*(x.data_ptr() for x in states))
+        a.buffers = C.cast(pointers, C.POINTER(C.c_void_p))
+        a.row_stride = int(first.stride(0)) * esz if R > 1 else 0
+        a.plane_stride, a.position_bytes, a.positions = plane_stride * esz, width * esz, positions
+        a.parents = self._device_tensor("parents", parents, torch.int32, R)
+        if lens is not None:
+            a.lens = self._device_tensor("lens", lens, torch.int32, R // beams)
+        return PreparedCall(self, states, self._lib.born_beam_reorder, a, (states, pointers, parents, lens))
+
+    def beam_reorder(self, states, parents, beams, lens=None, position_dim=None, stream=None):
+        """In every state [groups * beams, ...], row n * beams + b becomes, in place, what row
+        n * beams + parents[n * beams + b] was.  With `lens` [groups] only the first lens[n] entries of
+        dimension `position_dim` move (an attention cache's positions in use)."""
+        return self.prepare_beam_reorder(states, parents, beams, lens=lens, position_dim=position_dim).run(stream)
+
+    def prepare_beam_sequences(self, tokens, parents, end_step, end_parent, end_token, beams, pad=-1, out=None):
+        """Marshal a `beam_sequences` call once."""
+        if not _on_device(tokens) or tokens.ndim != 2 or not _on_device(parents) or parents.shape != tokens.shape:
+            raise InvalidArgument("beam_sequences: tokens and parents must be CUDA tensors [steps, groups * beams]")
+        T, R = (int(n) for n in tokens.shape)
+        beams = int(beams)
+        if beams < 1 or R % beams:
+            raise InvalidArgument(f"{R} rows are not a multiple of {beams} beams")
+        if getattr(end_step, "ndim", 0) != 2 or int(end_step.shape[0]) != R // beams:
+            raise InvalidArgument("beam_sequences: end_step must be [groups, hypotheses]")
+        H = int(end_step.shape[1])
+        a = L.SequencesArgs()
+        a.struct_size, a.memory = C.sizeof(L.SequencesArgs), L.MEM_DEVICE
+        a.groups, a.beams, a.steps, a.hypotheses, a.table_stride = R // beams, beams, T, H, R
+        a.tokens = self._device_tensor("tokens", tokens, torch.int32)
+        a.parents = self._device_tensor("parents", parents, torch.int32)
+        for name, x in (("end_step", end_step), ("end_parent", end_parent), ("end_token", end_token)):
+            setattr(a, name, self._device_tensor(name, x, torch.int32, R // beams * H))
+        res = out if out is not None else {}
+        if "tokens" not in res:
+            res["tokens"] = torch.empty((R // beams, H, T), dtype=torch.int32, device=tokens.device)
+        if "lens" not in res:
+            res["lens"] = torch.empty((R // beams, H), dtype=torch.int32, device=tokens.device)
+        a.out_tokens = self._device_tensor("out tokens", res["tokens"], torch.int32, R // beams * H * T)
+        a.out_lens = self._device_tensor("out lens", res["lens"], torch.int32, R // beams * H)
+        a.out_stride, a.pad = T, int(pad)
+        return PreparedCall(self, res, self._lib.born_beam_sequences, a,
+                            (tokens, parents, end_step, end_parent, end_token))
+
+    def beam_sequences(self, tokens, parents, end_step, end_parent, end_token, beams, pad=-1, out=None, stream=None):
+        """Sequences of hypotheses (step, parent, token) [groups, hypotheses], as a pool holds them, out of the
+        tables [steps, groups * beams] of the tokens and parents that the steps returned: tokens
+        [groups, hypotheses, steps] padded with `pad`, and lens [groups, hypotheses]."""
+        return self.prepare_beam_sequences(tokens, parents, end_step, end_parent, end_token, beams, pad, out).run(stream)
 
     # -- vocab-sharded path ---------------------------------------------------------------
     def record_bytes(self, top_k):

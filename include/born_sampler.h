@@ -59,7 +59,9 @@ extern "C" {
 #define BORN_ROW_OVERFLOW 4   /* only from born_shard_merge: the gathered records hold more than BORN_MAX_CANDIDATES tokens */
 #define BORN_ROW_BAD_TOKEN 5  /* speculative verify: draft token outside [0, vocab) */
 #define BORN_ROW_BAD_PARAMS 7 /* a row of a device-resident row_params array is out of range: token = -1 */
-#define BORN_ROW_FINISHED 6   /* born_sample_next: the row sampled a stop token in an earlier step; token = -1 */
+#define BORN_ROW_FINISHED 6   /* born_sample_next: the row sampled a stop token in an earlier step; token = -1.
+                                 born_beam_step: the group is done (see born_beam_args.done) */
+#define BORN_ROW_DEAD 8       /* born_beam_step: the row's score is -inf, it has no candidates */
 
 /* ---- limits ---- */
 #define BORN_MAX_TOP_K 1024
@@ -68,6 +70,10 @@ extern "C" {
 #define BORN_MAX_VOCAB ((1 << 24) - 4096)
 #define BORN_MAX_DRAFT 16          /* speculative draft length */
 #define BORN_MAX_SHARDS 16
+#define BORN_MAX_BEAMS 16          /* beams of a group */
+#define BORN_MAX_STOPS 8           /* stop tokens */
+#define BORN_MAX_REORDER 128       /* buffers of one born_beam_reorder call */
+#define BORN_MAX_STEPS 16384       /* steps of the tables that born_beam_sequences reads */
 
 #define BORN_DTYPE_F32 0
 #define BORN_DTYPE_BF16 1
@@ -305,6 +311,130 @@ int32_t born_sample_next(void* handle, const born_sample_args* args, void* strea
 int32_t born_mask_begin(void* handle, int32_t batch, int32_t words_per_row, uint32_t** host_buffer);
 int32_t born_mask_commit(void* handle, const uint32_t** device_mask);
 int32_t born_mask_wait(void* handle, void* stream);
+
+/* ---- beam search ------------------------------------------------------------------------
+ * Search in place of sampling over the same logits rows.  Row n*beams + b of every array belongs
+ * to beam b of group (sequence) n.  A step of the loop: the caller's model makes
+ * the logits, born_beam_step picks the beams that go on, born_beam_reorder moves the caller's
+ * per-beam states (attention caches, recurrent states) after them; at the end
+ * born_beam_sequences reads the token sequences out of the tables that the steps wrote.  All
+ * entry points take device memory, are asynchronous on `stream`, allocate nothing and can be
+ * captured in a CUDA graph.  The row arithmetic is the max-shifted log-softmax of
+ * internal/nn/cross_entropy.go:126-153; the search itself has no counterpart in the reference. */
+
+#define BORN_BEAM_KEEP_SLOTS 1u /* the best child of a beam stays in the beam's own row, the other children take the
+                                   rows of beams that end: fewer states move.  Without it children are in rank order */
+#define BORN_BEAM_EARLY_STOP 2u /* a group is done as soon as its pool is full */
+
+/* Arguments of born_beam_step.  For every row: penalties and mask as in born_sample, then
+ *     s[b][t] = scores[b] + z[t]/T - log sum_j exp(z[j]/T)        (tokens at -inf are no candidates)
+ * Candidates of a group are ranked by s in 64 bits, equal ones by b*vocab + t ascending.  The best
+ * `beams` that are no stop tokens go on; stop tokens among the best `beams` of all candidates end.
+ * A row whose score is -inf (BORN_ROW_DEAD), or whose status is not BORN_ROW_OK, has no candidates and does not
+ * stop the others.  Where fewer than `beams` candidates go on, the remaining rows get parent = the
+ * row's own beam, token -1, score -inf.  out_score may be the array `scores` points to. */
+typedef struct born_beam_args {
+    uint32_t struct_size; /* sizeof(born_beam_args) */
+    uint32_t memory;      /* BORN_MEM_DEVICE */
+    int32_t groups;       /* groups * beams <= the handle's max_batch */
+    int32_t beams;        /* 1..BORN_MAX_BEAMS */
+    int32_t vocab;
+    int32_t logits_dtype;
+    int64_t logits_row_stride; /* elements */
+    const void* logits;        /* [groups*beams, logits_row_stride] */
+    const uint32_t* mask;      /* [groups*beams, mask_row_stride] as in born_sample_args; NULL = none */
+    int64_t mask_row_stride;
+    const int32_t* history;     /* [groups*beams, history_stride]; NULL = none */
+    const int32_t* history_len; /* [groups*beams]; NULL = history_stride */
+    int32_t history_stride;     /* <= BORN_MAX_HISTORY */
+    uint32_t flags;             /* BORN_BEAM_* */
+    born_row_params params;     /* temperature (0 => 1) and the penalties; top_k, top_p, min_p and flags must be 0 */
+    const float* scores;        /* [groups*beams] log-probability of every beam so far; -inf = no such beam */
+    int32_t stop_ids[BORN_MAX_STOPS];
+    int32_t n_stop;
+    int32_t step;               /* 0-based; a hypothesis that ends in this step has step + 1 tokens (pool only) */
+    int32_t* out_parent; /* [groups*beams] beam (0..beams-1) of the same group that the row continues */
+    int32_t* out_token;  /* [groups*beams] its token, -1 = none */
+    float* out_score;    /* [groups*beams] */
+    int32_t* out_status; /* [groups*beams] BORN_ROW_* of the logits row that was read; NULL = skip */
+    int32_t* out_end_parent; /* [groups*beams] hypotheses that end in this step, best first, -1 padded; NULL = skip (all three) */
+    int32_t* out_end_token;
+    float* out_end_score;    /* ... their log-probabilities, -inf padded */
+    /* The pool: the best `beams` ended hypotheses of every group over all steps, updated in place;
+     * all five NULL = none.  born_beam_pool_reset empties it.  Sorted by score / length^length_penalty
+     * descending, an earlier entry before a later equal one. */
+    float* pool_score;    /* [groups*beams] normalised, -inf = free */
+    int32_t* pool_step;   /* [groups*beams] step in which it ended, -1 = free */
+    int32_t* pool_parent; /* [groups*beams] beam that it ended from */
+    int32_t* pool_token;  /* [groups*beams] the stop token */
+    /* [groups] set when the pool is full and no beam that goes on is, normalised at its present
+     * length, better than the pool's last entry (or BORN_BEAM_EARLY_STOP), or when no beam goes on.
+     * A group that is done reads no logits: parent = the row's own beam, token -1, score -inf,
+     * status BORN_ROW_FINISHED. */
+    int32_t* done;
+    float length_penalty; /* 0 => scores are compared as they are */
+    int32_t reserved;
+} born_beam_args;
+
+/* One launch: every logit is read once.  Candidates are collected while the rows stream and ranked
+ * by the CTA of a group that comes last. */
+int32_t born_beam_step(void* handle, const born_beam_args* args, void* stream);
+
+/* born_beam_step over the device-resident history (born_history_create / _reset with a row per
+ * beam): args->history and args->history_len must be NULL.  The kernel moves the histories after
+ * the beams that go on and appends their tokens.  Stop tokens are those of the arguments. */
+int32_t born_beam_next(void* handle, const born_beam_args* args, void* stream);
+
+/* Empties a pool: scores -inf, steps, parents and tokens -1, done 0. */
+int32_t born_beam_pool_reset(void* handle, const born_beam_args* args, void* stream);
+
+/* Arguments of born_beam_reorder: in every buffer, row n*beams + b becomes what row
+ * n*beams + parents[n*beams + b] was, in place; a parent outside 0..beams-1 leaves the row as it is.
+ * A row is `planes` pieces (heads, layers) of `positions` positions of position_bytes contiguous
+ * bytes; only the first lens[n] positions move, what lies behind them stays.  Buffers must not overlap. */
+typedef struct born_reorder_args {
+    uint32_t struct_size;
+    uint32_t memory; /* BORN_MEM_DEVICE: the buffers, parents, lens; `buffers` itself is a host array */
+    int32_t groups;
+    int32_t beams;
+    int32_t n_buffers; /* 1..BORN_MAX_REORDER, all of the same layout */
+    int32_t planes;
+    void* const* buffers;
+    int64_t row_stride;     /* bytes between rows */
+    int64_t plane_stride;   /* bytes between the pieces of a row */
+    int64_t position_bytes;
+    int64_t positions;
+    const int32_t* parents; /* [groups*beams] */
+    const int32_t* lens;    /* [groups] positions in use, clamped to 0..positions; NULL = positions */
+} born_reorder_args;
+int32_t born_beam_reorder(void* handle, const born_reorder_args* args, void* stream);
+
+/* Arguments of born_beam_sequences.  tokens / parents are the tables of `steps` rows that the steps
+ * wrote (out_token, out_parent of step t in row t).  A hypothesis is (step, parent, token) as the pool
+ * holds it: it ends in `token` at `step`, before that it follows beam `parent` back.  A beam that is
+ * still going is (step, out_parent, out_token) of the last step.  step outside 0..steps-1, or a parent outside
+ * 0..beams-1 on the way, gives an empty sequence (length 0). */
+typedef struct born_sequences_args {
+    uint32_t struct_size;
+    uint32_t memory; /* BORN_MEM_DEVICE */
+    int32_t groups;
+    int32_t beams;
+    int32_t steps;
+    int32_t hypotheses;      /* per group, 1..BORN_MAX_BEAMS */
+    int64_t table_stride;    /* elements between the rows of the tables (>= groups*beams) */
+    const int32_t* tokens;   /* [steps, table_stride] */
+    const int32_t* parents;  /* [steps, table_stride] */
+    const int32_t* end_step;   /* [groups, hypotheses] */
+    const int32_t* end_parent; /* [groups, hypotheses] */
+    const int32_t* end_token;  /* [groups, hypotheses] */
+    int32_t* out_tokens;       /* [groups, hypotheses, out_stride]: the first `steps` of a row are
+                                  written, those from the sequence's length on as `pad` */
+    int64_t out_stride;        /* >= steps */
+    int32_t* out_lens;         /* [groups, hypotheses] */
+    int32_t pad;
+    int32_t reserved;
+} born_sequences_args;
+int32_t born_beam_sequences(void* handle, const born_sequences_args* args, void* stream);
 
 /* Test hooks: run the library's deterministic exp / fixed-point mass on device arrays. */
 int32_t born_debug_exp(const float* x_dev, float* y_dev, int64_t n, void* stream);
