@@ -30,6 +30,7 @@ FLAG_GREEDY = 1
 FLAG_FULL_VOCAB = 2
 BEAM_KEEP_SLOTS = 1
 BEAM_EARLY_STOP = 2
+ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "gelu": 4, "silu": 5}
 
 
 class RowParams(C.Structure):
@@ -196,6 +197,28 @@ class SequencesArgs(C.Structure):
     ]
 
 
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("memory", C.c_uint32),
+        ("rows", C.c_int32),
+        ("hidden", C.c_int32),
+        ("features", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("activation", C.c_int32),
+        ("scale", C.c_float),
+        ("x", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("out", C.c_void_p),
+        ("x_row_stride", C.c_int64),
+        ("weight_row_stride", C.c_int64),
+        ("residual_row_stride", C.c_int64),
+        ("out_row_stride", C.c_int64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/born_sampler.h
 SYMBOLS = {
     "born_sampler_create": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
@@ -220,6 +243,7 @@ SYMBOLS = {
     "born_beam_pool_reset": (C.c_int32, [C.c_void_p, C.POINTER(BeamArgs), C.c_void_p]),
     "born_beam_reorder": (C.c_int32, [C.c_void_p, C.POINTER(ReorderArgs), C.c_void_p]),
     "born_beam_sequences": (C.c_int32, [C.c_void_p, C.POINTER(SequencesArgs), C.c_void_p]),
+    "born_linear": (C.c_int32, [C.c_void_p, C.POINTER(LinearArgs), C.c_void_p]),
     "born_shard_record_bytes": (C.c_int32, [C.c_int32]),
     "born_shard_unique_id": (C.c_int32, [C.c_void_p]),
     "born_shard_init": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32]),

@@ -20,6 +20,7 @@
 #include "prepass.cuh"
 #include "spec_kernel.cuh"
 #include "beam_launch.cuh"
+#include "linear_launch.cuh"
 
 using namespace born;
 
@@ -435,7 +436,7 @@ int32_t born_sampler_create(int32_t device, int32_t max_batch, int32_t max_vocab
     if (rc == BORN_OK && scan_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cluster_limits(h->max_clusters) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && spec_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
-    if (rc == BORN_OK && (beam_attrs() != cudaSuccess || sequences_attrs() != cudaSuccess)) rc = BORN_ERR_CUDA;
+    if (rc == BORN_OK && (beam_attrs() != cudaSuccess || sequences_attrs() != cudaSuccess || linear_attrs() != cudaSuccess)) rc = BORN_ERR_CUDA;
     for (int i = 0; i < 4 && rc == BORN_OK; ++i)
         if (cudaEventCreate(&h->ev[i]) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc != BORN_OK) {
@@ -1267,6 +1268,44 @@ int32_t born_beam_sequences(void* handle, const born_sequences_args* a, void* st
     A.end_step = a->end_step; A.end_parent = a->end_parent; A.end_token = a->end_token;
     A.out_tokens = a->out_tokens; A.out_lens = a->out_lens; A.pad = a->pad;
     CUDA_TRY(h, sequences_launch(A, (cudaStream_t)stream));
+    h->launches++;
+    return BORN_OK;
+}
+
+// ------------------------------------------------------------------ the output head
+int32_t born_linear(void* handle, const born_linear_args* a, void* stream) {
+    Handle* h = (Handle*)handle;
+    if (!h) return fail(nullptr, BORN_ERR_INVALID_ARGUMENT, "handle is NULL");
+    const int rc = args_check(h, a, "linear");
+    if (rc) return rc;
+    if (a->rows < 1 || a->hidden < 1 || a->features < 1)
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: rows %d, hidden %d and features %d must be positive", a->rows, a->hidden, a->features);
+    if (a->out_dtype != BORN_DTYPE_F32 && a->out_dtype != BORN_DTYPE_BF16) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: unknown out_dtype %d", a->out_dtype);
+    if (a->activation < BORN_ACT_NONE || a->activation > BORN_ACT_SILU) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: unknown activation %d", a->activation);
+    if (!(a->scale >= 0.0f) || !isfinite(a->scale)) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: scale out of range");
+    if (!a->x || !a->weight || !a->out) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: x, weight and out are required");
+    if (a->x_row_stride < a->hidden || a->weight_row_stride < a->hidden || a->out_row_stride < a->features ||
+        (a->residual && a->residual_row_stride < a->features))
+        return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: a row stride is shorter than its row");
+    const size_t esz = a->out_dtype == BORN_DTYPE_F32 ? 4 : 2;
+    if (unaligned(a->out, esz) || unaligned(a->residual, esz) || unaligned(a->bias, 4)) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: a pointer is not aligned to its element size");
+    // the operands are read as TMA tiles
+    if (a->hidden % 8 || a->x_row_stride % 8 || a->weight_row_stride % 8 || unaligned(a->x, 16) || unaligned(a->weight, 16))
+        return fail(h, BORN_ERR_UNSUPPORTED, "linear: hidden must be a multiple of 8, rows of x and weight start on 16-byte boundaries");
+    if (a->x_row_stride >= (1ll << 39) || a->weight_row_stride >= (1ll << 39)) return fail(h, BORN_ERR_UNSUPPORTED, "linear: row stride too long");
+    DeviceScope on(h);
+    if (on.rc) return on.rc;
+    LinearArgs A;
+    memset(&A, 0, sizeof A);
+    A.M = a->rows; A.K = a->hidden; A.V = a->features;
+    A.activation = a->activation;
+    A.scale = a->scale == 0.0f ? 1.0f : a->scale;
+    A.x = a->x; A.weight = a->weight; A.bias = a->bias; A.residual = a->residual; A.out = a->out;
+    A.x_stride = a->x_row_stride; A.weight_stride = a->weight_row_stride;
+    A.residual_stride = a->residual_row_stride; A.out_stride = a->out_row_stride;
+    A.dev_error = h->dev_error;
+    A.timeout_ns = h->timeout_ns;
+    CUDA_TRY(h, linear_launch(A, a->out_dtype, h->num_sms, (cudaStream_t)stream));
     h->launches++;
     return BORN_OK;
 }

@@ -658,6 +658,50 @@ class Sampler:
         [groups, hypotheses, steps] padded with `pad`, and lens [groups, hypotheses]."""
         return self.prepare_beam_sequences(tokens, parents, end_step, end_parent, end_token, beams, pad, out).run(stream)
 
+    # -- the output head ----------------------------------------------------------------------
+    def prepare_linear(self, x, weight, bias=None, residual=None, activation="none", scale=1.0, out_dtype=None, out=None):
+        """Marshal a `linear` call once."""
+        for name, t in (("x", x), ("weight", weight)):
+            if getattr(t, "ndim", 0) != 2:
+                raise InvalidArgument(f"linear: {name} must be 2D")
+            self._device_tensor(name, t, torch.bfloat16, contiguous=False)
+            if t.stride(1) != 1:
+                raise InvalidArgument(f"linear: {name} rows must be contiguous")
+        M, H = (int(n) for n in x.shape)
+        V = int(weight.shape[0])
+        if int(weight.shape[1]) != H:
+            raise InvalidArgument(f"linear: weight is {tuple(weight.shape)}, x {tuple(x.shape)}")
+        if activation not in L.ACTIVATIONS:
+            raise InvalidArgument(f"linear: unknown activation {activation!r}")
+        if out is None:
+            out = torch.empty((M, V), dtype=out_dtype or torch.float32, device=x.device)
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise InvalidArgument(f"linear: out is {out.dtype}, not {out_dtype}")
+        a = L.LinearArgs()
+        a.struct_size, a.memory = C.sizeof(L.LinearArgs), L.MEM_DEVICE
+        a.rows, a.hidden, a.features = M, H, V
+        a.out_dtype = _logits_dtype(out, False)
+        for name, t in (("out", out), ("residual", residual)):
+            if t is None:
+                continue
+            self._device_tensor(name, t, out.dtype, contiguous=False)
+            if tuple(t.shape) != (M, V) or (V > 1 and t.stride(1) != 1):
+                raise InvalidArgument(f"linear: {name} must be [{M}, {V}] with contiguous rows")
+            setattr(a, name, t.data_ptr())
+            setattr(a, name + "_row_stride", int(t.stride(0)) if M > 1 else V)
+        if bias is not None:
+            a.bias = self._device_tensor("bias", bias, torch.float32, V)
+        a.x, a.x_row_stride = x.data_ptr(), int(x.stride(0)) if M > 1 else H
+        a.weight, a.weight_row_stride = weight.data_ptr(), int(weight.stride(0)) if V > 1 else H
+        a.activation, a.scale = L.ACTIVATIONS[activation], float(scale)
+        return PreparedCall(self, out, self._lib.born_linear, a, (x, weight, bias, residual))
+
+    def linear(self, x, weight, bias=None, residual=None, activation="none", scale=1.0, out_dtype=None, out=None, stream=None):
+        """act(x [rows, hidden] weight [features, hidden]^T + bias [features]) + residual [rows, features]: the
+        layer that makes the logits.  x and weight bf16, bias fp32, residual and result fp32 (default) or bf16.
+        activation: none, relu, sigmoid, tanh (scale * tanh(y / scale), which caps logits), gelu, silu."""
+        return self.prepare_linear(x, weight, bias, residual, activation, scale, out_dtype, out).run(stream)
+
     # -- vocab-sharded path ---------------------------------------------------------------
     def record_bytes(self, top_k):
         return int(self._lib.born_shard_record_bytes(int(top_k)))

@@ -314,7 +314,7 @@ int32_t born_mask_wait(void* handle, void* stream);
 
 /* ---- beam search ------------------------------------------------------------------------
  * Search in place of sampling over the same logits rows.  Row n*beams + b of every array belongs
- * to beam b of group (sequence) n.  A step of the loop: the caller's model makes
+ * to beam b of group (sequence) n.  A step of the loop: born_linear (or the caller's model) makes
  * the logits, born_beam_step picks the beams that go on, born_beam_reorder moves the caller's
  * per-beam states (attention caches, recurrent states) after them; at the end
  * born_beam_sequences reads the token sequences out of the tables that the steps wrote.  All
@@ -435,6 +435,39 @@ typedef struct born_sequences_args {
     int32_t reserved;
 } born_sequences_args;
 int32_t born_beam_sequences(void* handle, const born_sequences_args* args, void* stream);
+
+/* ---- the output head ----------------------------------------------------------------------
+ * out[m][v] = act(sum_k x[m][k] * weight[v][k] + bias[v]) + residual[m][v]: the layer in front of
+ * the sampler (internal/nn/linear.go:78-107 with the activations of
+ * internal/nn/activation.go:7-20), whose output born_sample and born_beam_step read.  bf16
+ * operands, fp32 accumulation, one rounding to the output type after the epilogue. */
+#define BORN_ACT_NONE 0
+#define BORN_ACT_RELU 1
+#define BORN_ACT_SIGMOID 2
+#define BORN_ACT_TANH 3 /* scale * tanh(y / scale): caps logits at +-scale */
+#define BORN_ACT_GELU 4 /* 0.5 y (1 + erf(y / sqrt 2)) */
+#define BORN_ACT_SILU 5
+
+typedef struct born_linear_args {
+    uint32_t struct_size;
+    uint32_t memory;   /* BORN_MEM_DEVICE */
+    int32_t rows;      /* m */
+    int32_t hidden;    /* k, a multiple of 8 */
+    int32_t features;  /* v */
+    int32_t out_dtype; /* BORN_DTYPE_* of out and residual */
+    int32_t activation; /* BORN_ACT_* */
+    float scale;        /* BORN_ACT_TANH: > 0 (0 => 1) */
+    const void* x;           /* [rows, x_row_stride] bf16 */
+    const void* weight;      /* [features, weight_row_stride] bf16 */
+    const float* bias;       /* [features] fp32; NULL = none */
+    const void* residual;    /* [rows, residual_row_stride]; NULL = none; may be `out` */
+    void* out;               /* [rows, out_row_stride] */
+    int64_t x_row_stride;    /* elements; x and weight rows start on 16-byte boundaries */
+    int64_t weight_row_stride;
+    int64_t residual_row_stride;
+    int64_t out_row_stride;
+} born_linear_args;
+int32_t born_linear(void* handle, const born_linear_args* args, void* stream);
 
 /* Test hooks: run the library's deterministic exp / fixed-point mass on device arrays. */
 int32_t born_debug_exp(const float* x_dev, float* y_dev, int64_t n, void* stream);
