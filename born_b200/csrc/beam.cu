@@ -1,65 +1,101 @@
 // Beam search (step, reordering of states, read-out of sequences): instantiations and launches.
+#include <string.h>
 #include "beam_kernel.cuh"
 #include "reorder_kernel.cuh"
 #include "sequences_kernel.cuh"
 
 namespace born {
 
-// A slice's bits fill at most 37.5 KB of shared memory.
-static int least_slices(int vocab) { return (vocab + 299999) / 300000; }
-
-// Slices of at least 4096 tokens, as many as give every SM four CTAs.
-int beam_slices(int rows, int vocab, int num_sms) {
-    int s = (4 * num_sms + rows - 1) / rows;
-    const int most = (vocab + 4095) / 4096;
-    if (s > most) s = most;
-    if (s > kBeamMaxSlices) s = kBeamMaxSlices;
-    const int least = least_slices(vocab);
-    if (s < least) s = least;
-    return s < 1 ? 1 : s;
+static void row_pieces(int vocab, int& pieces, int& pb) {
+    const int nb = (vocab + kBlkTok - 1) / kBlkTok;
+    pieces = (nb + kBeamPiece - 1) / kBeamPiece;
+    pb = (nb + pieces - 1) / pieces;
 }
 int64_t beam_max_records(int max_batch, int max_vocab, int num_sms) {
-    // rows * beam_slices(rows): less than 4 CTAs per SM and one more per row, or the least slices of every row
-    const int64_t fill = 4 * (int64_t)num_sms + max_batch, least = (int64_t)max_batch * least_slices(max_vocab);
-    return fill > least ? fill : least;
+    int pieces, pb;
+    row_pieces(max_vocab, pieces, pb);
+    return 2 * (int64_t)num_sms + (int64_t)max_batch * (pieces + 1);  // (CTAs and pieces; a CTA of its own for every piece)
 }
 
-// The normaliser log sum exp of a row in 32 bits.  Every value's exponent t (base 2, relative to a maximum
-// that may be 2^8 behind) rounds by 2^-24 |t| in the subtraction, in the scaling and through the scale's own
-// rounding, and sum p |t| <= log2(V) + 8; ex2 is off by 2^-22, once per value and once per thread;
-// a thread's sum rounds once per turn of 16 values after a tree of 16.  The rest is in 64 bits.
-static double beam_slack(int vocab, int slices) {
+// What the normalisers log sum exp of two rows are off by at most in 32 bits (BeamSum): every value by ex2's
+// 2^-22 and 2^-25 of the fraction in the exponent, sums of 32 by their six rounded additions; the rest is in 64 bits.
+static double beam_slack() {
     const double u = ldexp(1.0, -24);
-    const double turns = (double)vocab / slices / (16.0 * kThreads) + 8.0;
-    const double one = 3 * u * (log2((double)vocab) + 8.0) * M_LN2 + 8 * u + (turns + 4.0) * u;
-    return 2.0 * one;
+    return 2.0 * (4 * u + 0.5 * u + 6 * u + 0.5 * u);
 }
 
-template <typename T, bool kBits>
+// Dynamic shared memory of a CTA, two of which share an SM's 228 KB.
+constexpr int kBeamSmem = (228 * 1024 / 2 - 1024 - (int)sizeof(BeamShared) - 8 * kBeamWarps * kBeamMaxSlots - 16) & ~127;
+template <typename T, bool kBits, bool kAligned>
 static cudaError_t raise_limit() {
-    return cudaFuncSetAttribute(beam_kernel<T, kBits>, cudaFuncAttributeMaxDynamicSharedMemorySize, 40 * 1024);
+    return cudaFuncSetAttribute(beam_kernel<T, kBits, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamSmem);
+}
+template <typename T>
+static cudaError_t raise_limits() {
+    cudaError_t e;
+    if ((e = raise_limit<T, false, false>()) != cudaSuccess || (e = raise_limit<T, false, true>()) != cudaSuccess) return e;
+    if ((e = raise_limit<T, true, false>()) != cudaSuccess) return e;
+    return raise_limit<T, true, true>();
 }
 cudaError_t beam_attrs() {
-    cudaError_t e = raise_limit<float, true>();
-    return e != cudaSuccess ? e : raise_limit<uint16_t, true>();
+    const cudaError_t e = raise_limits<float>();
+    return e != cudaSuccess ? e : raise_limits<uint16_t>();
 }
 
-cudaError_t beam_launch(BeamArgs& A, int dtype, cudaStream_t st) {
-    const int grid = A.N * A.K * A.slices;
+// A launch that may begin while the one before it ends (the kernels wait before they read).
+template <typename... P, typename... Q>
+static cudaError_t launch_after(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, const Q&... args) {
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3((unsigned)threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T>
+static cudaError_t beam_launch_as(const BeamArgs& A, bool has_bits, bool aligned, size_t smem, cudaStream_t st) {
+    const unsigned grid = (unsigned)A.grid;
+    if (has_bits)
+        return aligned ? launch_after(beam_kernel<T, true, true>, grid, kThreads, smem, st, A) : launch_after(beam_kernel<T, true, false>, grid, kThreads, smem, st, A);
+    return aligned ? launch_after(beam_kernel<T, false, true>, grid, kThreads, smem, st, A) : launch_after(beam_kernel<T, false, false>, grid, kThreads, smem, st, A);
+}
+
+cudaError_t beam_launch(BeamArgs& A, int dtype, bool aligned, int num_sms, cudaStream_t st) {
     const bool has_bits = A.mask || A.history;
-    // vectors per slice, rounded up, and the two words of the tokens beside them
-    const int vec = dtype == BORN_DTYPE_F32 ? 4 : 8;
-    A.bit_words = has_bits ? ((A.V / vec + A.slices) / A.slices * vec + 31) / 32 + 2 : 0;
-    A.slack = beam_slack(A.V, A.slices);
-    const size_t smem = (size_t)A.bit_words * 4;
-    if (dtype == BORN_DTYPE_F32) {
-        if (has_bits) beam_kernel<float, true><<<grid, kThreads, smem, st>>>(A);
-        else beam_kernel<float, false><<<grid, kThreads, 0, st>>>(A);
-    } else {
-        if (has_bits) beam_kernel<uint16_t, true><<<grid, kThreads, smem, st>>>(A);
-        else beam_kernel<uint16_t, false><<<grid, kThreads, 0, st>>>(A);
-    }
-    return cudaGetLastError();
+    row_pieces(A.V, A.pieces, A.pb);
+    const int64_t rows = (int64_t)A.N * A.K, pieces = rows * A.pieces, blocks = pieces * A.pb;
+    if (blocks > 0x7fffffff / kBlkTok) return cudaErrorInvalidValue;
+    A.blocks = (int)blocks;
+    // a block per warp at least, a CTA of its own for every piece while the GPU holds them at once
+    int64_t grid = (blocks + kBeamWarps - 1) / kBeamWarps;
+    if (grid < pieces) grid = pieces;
+    if (grid > 2 * num_sms) grid = 2 * num_sms;
+    A.grid = (int)grid;
+    const int range = (int)((blocks + grid - 1) / grid), seg = range < kBeamSegs * A.pb ? range : kBeamSegs * A.pb;  // blocks taken at a time
+    const int esz = dtype == BORN_DTYPE_F32 ? 4 : 2;
+    const int bit_bytes = has_bits ? seg * 128 : 0, key_bytes = (seg * 64 + 127) & ~127;
+    A.bit_words = bit_bytes / 4;
+    A.slot_bytes = ring_slot_bytes(esz, aligned);
+    A.hist_cap = A.history ? (A.history_stride + 31) / 32 * 32 : 0;  // ids, penalised logits and later occurrences of each segment
+    const int hist_bytes = kBeamSegs * A.hist_cap * 12;
+    A.slots = (kBeamSmem - bit_bytes - key_bytes - hist_bytes) / (kBeamWarps * A.slot_bytes);
+    const int most = (range + kBeamWarps - 1) / kBeamWarps;
+    if (A.slots > most) A.slots = most;
+    if (A.slots > kBeamMaxSlots) A.slots = kBeamMaxSlots;
+    A.bits_at = kBeamWarps * A.slots * A.slot_bytes;
+    A.gkeys_at = A.bits_at + bit_bytes;
+    A.slack = beam_slack();
+    A.hist_at = A.gkeys_at + key_bytes;
+    const size_t smem = (size_t)A.hist_at + hist_bytes;
+    if (dtype == BORN_DTYPE_F32) return beam_launch_as<float>(A, has_bits, aligned, smem, st);
+    return beam_launch_as<uint16_t>(A, has_bits, aligned, smem, st);
 }
 
 // The widest vectors that every row and piece is aligned to; ranges of 32 KB a CTA, smaller ones where

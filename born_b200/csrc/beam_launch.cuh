@@ -6,19 +6,27 @@
 
 namespace born {
 
-constexpr int kBeamMaxSlices = 64;    // slices of a row: two records per lane of the warp that merges them
+constexpr int kBeamPiece = 128;     // blocks of a piece of a row: 16 KB of bits, 8 KB of group keys
+constexpr int kBeamMaxSlots = 8;    // ring slots of a warp
 
-// What a slice leaves for the merge.
+// What a segment leaves for the merge.
 struct BeamRecord {
-    double sum;  // sum exp((z - max)/T) over the slice
-    float max;   // NaN / +inf: the slice holds one
-    uint32_t pad;
-    float stop_z[BORN_MAX_STOPS];  // penalised logits of the stop tokens in the slice, -inf elsewhere
+    double sum;  // sum exp(z/T) over the segment, in units of 2^m exp(z0/T)
+    int32_t m;   // INT_MIN: nothing
+    float z0;
+    float max;   // NaN / +inf: the segment holds one
+    int32_t failed;  // a wait for a copy ran out
+    int32_t pad[2];
+    float stop_z[BORN_MAX_STOPS];  // penalised logits of the stop tokens in the segment, -inf elsewhere
     unsigned long long list[BORN_MAX_BEAMS];  // rank keys of the best tokens, 0 = none
 };
 
 struct BeamArgs {
-    int N, K, V, slices;
+    int N, K, V;
+    // A row is `pieces` pieces of `pb` blocks of 1024 tokens (the last ones may be empty); the `blocks` blocks of
+    // all rows are dealt to `grid` CTAs in equal ranges.
+    int pieces, pb, blocks, grid;
+    int slots, slot_bytes, bits_at, gkeys_at, hist_at, hist_cap;  // shared memory
     const void* logits;
     int64_t row_stride;
     const uint32_t* mask;
@@ -28,7 +36,8 @@ struct BeamArgs {
     int history_stride;
     uint32_t flags;
     born_row_params params;
-    float temperature, scale_log2e;  // T; log2(e)/T
+    float temperature, scale_log2e, scale_lo;  // T; log2(e)/T in two parts
+    double inv_T;   // 1/T
     double slack;   // two normalisers in 32 bits are off by less than this together
     int bit_words;  // words of a CTA's bit map
     const float* scores;
@@ -45,17 +54,24 @@ struct BeamArgs {
     // workspace
     BeamRecord* records;
     uint32_t* tickets;
+    int* dev_error;
+    unsigned long long timeout_ns;
     // device-resident history (born_beam_next)
     int32_t *ring, *ring_total, *ring_len;
     int ring_cap;
+
+    // (blocks < 2^21, grid < 2^10)
+    __host__ __device__ int range_start(int cta) const { return (int)((unsigned)cta * (unsigned)blocks / (unsigned)grid); }
+    // A segment is a CTA and a piece; from one to the next the CTA or the piece goes up by one, or both, so their
+    // sum numbers the segments.  Of the segment that holds block t:
+    __host__ __device__ int record_of(int t) const { return (int)(((unsigned)(t + 1) * (unsigned)grid - 1u) / (unsigned)blocks) + t / pb; }
 };
 
-// Slices per row for a launch of `rows` rows.
-int beam_slices(int rows, int vocab, int num_sms);
 // Records that launches of up to max_batch rows of up to max_vocab tokens leave.
 int64_t beam_max_records(int max_batch, int max_vocab, int num_sms);
 cudaError_t beam_attrs();
-cudaError_t beam_launch(BeamArgs& A, int dtype, cudaStream_t st);
+// Fills in how the rows are dealt; cudaErrorInvalidValue where they are too many.
+cudaError_t beam_launch(BeamArgs& A, int dtype, bool aligned, int num_sms, cudaStream_t st);
 
 // ---- born_beam_reorder ------------------------------------------------------------------------
 struct ReorderArgs {

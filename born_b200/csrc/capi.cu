@@ -342,6 +342,7 @@ int check_device_error(Handle* h) {
     if (e) {
         // tickets of rows that were left unfinished must not leak into the next launch
         cudaMemset(h->tickets, 0, sizeof(uint32_t) * 2 * (size_t)h->max_rows);
+        if (h->beam_tickets) cudaMemset(h->beam_tickets, 0, sizeof(uint32_t) * (size_t)h->max_batch);
         cudaMemset(h->dev_error, 0, sizeof(int));
         return fail(h, BORN_ERR_DEVICE_TIMEOUT, "a bounded on-device wait gave up (code %d); outputs of that call are invalid", e);
     }
@@ -1124,8 +1125,6 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
     BeamArgs A;
     memset(&A, 0, sizeof A);
     A.N = a->groups; A.K = a->beams; A.V = a->vocab;
-    A.slices = beam_slices((int)rows, a->vocab, h->num_sms);
-    if (rows * A.slices > h->beam_records_cap) return fail(h, BORN_ERR_UNSUPPORTED, "batch x vocab exceeds the workspace");
     A.logits = a->logits; A.row_stride = a->logits_row_stride;
     A.mask = a->mask; A.mask_stride = a->mask_row_stride;
     A.params = a->params;
@@ -1135,6 +1134,8 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
     A.flags = a->flags;
     A.temperature = a->params.temperature == 0.0f ? 1.0f : a->params.temperature;
     A.scale_log2e = (float)(M_LOG2E / (double)A.temperature);
+    A.inv_T = 1.0 / (double)A.temperature;
+    A.scale_lo = (float)(M_LOG2E / (double)A.temperature - (double)A.scale_log2e);
     A.scores = a->scores;
     for (int i = 0; i < a->n_stop; ++i) {  // those of the vocabulary, each once
         const int32_t t = a->stop_ids[i];
@@ -1150,13 +1151,16 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
     A.length_norm = pow((double)a->step + 1.0, (double)a->length_penalty);
     A.records = h->beam_records;
     A.tickets = h->beam_tickets;
+    A.dev_error = h->dev_error;
+    A.timeout_ns = h->timeout_ns;
     if (ring) {
         A.ring = h->ring;
         A.ring_total = h->ring + (size_t)h->max_batch * h->ring_cap;
         A.ring_len = A.ring_total + h->max_batch;
         A.ring_cap = h->ring_cap;
     }
-    CUDA_TRY(h, beam_launch(A, a->logits_dtype, st));
+    const bool aligned = rows_aligned(1, a->vocab, a->logits_dtype, a->logits, rows > 1 ? a->logits_row_stride : 0);
+    CUDA_TRY(h, beam_launch(A, a->logits_dtype, aligned, h->num_sms, st));
     h->launches++;
     return BORN_OK;
 }
