@@ -23,7 +23,6 @@ MAX_SHARDS = 16
 MAX_BEAMS = 16
 MAX_STOPS = 8
 MAX_REORDER = 128
-MAX_STEPS = 16384
 DTYPE_F32, DTYPE_BF16 = 0, 1
 MEM_DEVICE, MEM_HOST = 0, 1
 FLAG_GREEDY = 1

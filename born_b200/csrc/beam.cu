@@ -111,19 +111,20 @@ cudaError_t reorder_launch(ReorderArgs& A, cudaStream_t st) {
     while (pieces * ((piece + A.chunk - 1) / A.chunk) > 0x7fffffff) A.chunk *= 2;
     A.chunks = (int)((piece + A.chunk - 1) / A.chunk);
     const unsigned grid = (unsigned)(pieces * A.chunks);
-    if (low % 16 == 0) reorder_kernel<uint4><<<grid, kReorderThreads, 0, st>>>(A);
-    else if (low % 4 == 0) reorder_kernel<uint32_t><<<grid, kReorderThreads, 0, st>>>(A);
-    else if (low % 2 == 0) reorder_kernel<uint16_t><<<grid, kReorderThreads, 0, st>>>(A);
-    else reorder_kernel<uint8_t><<<grid, kReorderThreads, 0, st>>>(A);
-    return cudaGetLastError();
+    if (low % 16 == 0) return launch_after(reorder_kernel<uint4>, grid, kReorderThreads, 0, st, A);
+    if (low % 4 == 0) return launch_after(reorder_kernel<uint32_t>, grid, kReorderThreads, 0, st, A);
+    if (low % 2 == 0) return launch_after(reorder_kernel<uint16_t>, grid, kReorderThreads, 0, st, A);
+    return launch_after(reorder_kernel<uint8_t>, grid, kReorderThreads, 0, st, A);
 }
 
-cudaError_t sequences_attrs() {
-    return cudaFuncSetAttribute(sequences_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 10 * kSequenceMaxSteps);
-}
-cudaError_t sequences_launch(const SequencesArgs& A, cudaStream_t st) {
-    sequences_kernel<<<A.N, kSeqThreads, (size_t)A.T * 10, st>>>(A);
-    return cudaGetLastError();
+constexpr int kSeqSmem = 222 * 1024;
+cudaError_t sequences_attrs() { return cudaFuncSetAttribute(sequences_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSeqSmem); }
+cudaError_t sequences_launch(SequencesArgs& A, cudaStream_t st) {
+    A.shift = 2;
+    while ((1 << A.shift) < A.K || (1 << A.shift) < A.H) ++A.shift;
+    A.tile = kSeqSmem / (6 << A.shift);  // a token and two bytes per beam
+    if (A.tile > A.T) A.tile = A.T;
+    return launch_after(sequences_kernel, (unsigned)A.N, kSeqThreads, (size_t)A.tile * (6 << A.shift), st, A);
 }
 
 }  // namespace born

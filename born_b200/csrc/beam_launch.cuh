@@ -86,15 +86,15 @@ struct ReorderArgs {
 cudaError_t reorder_launch(ReorderArgs& A, cudaStream_t st);
 
 // ---- born_beam_sequences ------------------------------------------------------------------------
-constexpr int kSequenceMaxSteps = 16384;  // the steps' maps fill 160 KB of shared memory
 struct SequencesArgs {
     int N, K, T, H;
     int64_t table_stride, out_stride;
     const int32_t *tokens, *parents, *end_step, *end_parent, *end_token;
     int32_t *out_tokens, *out_lens;
     int32_t pad;
+    int tile, shift;  // steps that shared memory holds at a time, 2^shift places each
 };
 cudaError_t sequences_attrs();
-cudaError_t sequences_launch(const SequencesArgs& A, cudaStream_t st);
+cudaError_t sequences_launch(SequencesArgs& A, cudaStream_t st);
 
 }  // namespace born

@@ -1257,8 +1257,7 @@ int32_t born_beam_sequences(void* handle, const born_sequences_args* a, void* st
     int rc = args_check(h, a, "beam_sequences");
     if (rc || (rc = groups_check(h, a->groups, a->beams, "beam_sequences"))) return rc;
     if (a->steps < 1 || a->hypotheses < 1) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_sequences: steps and hypotheses must be positive");
-    if (a->steps > BORN_MAX_STEPS || a->hypotheses > BORN_MAX_BEAMS)
-        return fail(h, BORN_ERR_UNSUPPORTED, "beam_sequences: %d steps / %d hypotheses exceed %d / %d", a->steps, a->hypotheses, BORN_MAX_STEPS, BORN_MAX_BEAMS);
+    if (a->hypotheses > BORN_MAX_BEAMS) return fail(h, BORN_ERR_UNSUPPORTED, "beam_sequences: %d hypotheses exceed %d", a->hypotheses, BORN_MAX_BEAMS);
     if (a->table_stride < (int64_t)a->groups * a->beams || a->out_stride < a->steps)
         return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_sequences: table_stride < groups x beams, or out_stride < steps");
     if (!a->tokens || !a->parents || !a->end_step || !a->end_parent || !a->end_token || !a->out_tokens || !a->out_lens)

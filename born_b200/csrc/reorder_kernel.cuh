@@ -39,7 +39,7 @@ __device__ __forceinline__ void move_bytes(uint8_t* base, int64_t row_stride, co
 }
 
 template <typename W>
-__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderArgs A) {
+__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderArgs A) {
     __shared__ int dst[BORN_MAX_BEAMS], src[BORN_MAX_BEAMS];
     __shared__ int n_moves;
     // (chunk, piece, buffer, group), the chunks of a piece first
@@ -50,6 +50,8 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderA
     i /= A.planes;
     const int buffer = (int)(i % A.n_buffers);
     const int n = (int)(i / A.n_buffers);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int64_t used = A.positions;
     if (A.lens) {
         const int64_t len = A.lens[n];

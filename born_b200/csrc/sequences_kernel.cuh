@@ -1,10 +1,14 @@
 // Sequences of hypotheses out of the tables that the steps of a beam search wrote.
 //
-// Following the parents back is a chain of dependent reads, one per step.  A step's parents are a map of
-// at most 16 beams to 16 beams, 64 bits; maps compose, so a CTA (one per group) cuts the steps into a
-// chunk per thread, composes each chunk's map, and from tables of the maps over 2, 4, 8, ... chunks
-// every thread learns in eight look-ups at which beam each hypothesis enters its chunk.  The walks inside
-// the chunks then run side by side.
+// Following the parents back is a chain of dependent reads, one per step: 4096 steps would take a
+// millisecond of latency.  A step's parents are a map of at most 16 beams to 16 beams, and maps compose.  So a CTA
+// (one per group) brings parents and tokens of a tile of steps into shared memory, cuts the steps into 64 chunks, a
+// half warp each, and composes every chunk's map; a lane per hypothesis walks over the 64 maps; then all chunks
+// are walked at once, and the tokens are picked and written along the steps.  Longer tables go tile by
+// tile, from the end.
+// Bound by the bytes that one SM takes in (a group's rows are short pieces of the tables' rows) and by the two
+// walks, some 40 cycles a step: 64 groups of 8 beams, 4096 steps take 47 us when every chunk reads its own
+// parents and tokens as it walks, 36 us with the parents alone in shared memory.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -12,128 +16,132 @@
 
 namespace born {
 
-constexpr int kSeqThreads = 256;
-constexpr int kSeqLevels = 8;
-constexpr unsigned long long kIdentity = 0xfedcba9876543210ull;
-
-// A map of beams: nibble b holds the beam that b came from; bit b of bad: it came from none.
-struct BeamMap {
-    unsigned long long to;
-    uint32_t bad;
-};
-__device__ __forceinline__ int map_at(unsigned long long to, int b) { return (int)(to >> (4 * b)) & 15; }
-// first `a` (later steps), then `b` (earlier ones)
-__device__ __forceinline__ BeamMap compose(const BeamMap& a, const BeamMap& b) {
-    BeamMap r;
-    r.to = 0;
-    r.bad = a.bad;
-#pragma unroll
-    for (int i = 0; i < BORN_MAX_BEAMS; ++i) {
-        const int m = map_at(a.to, i);
-        r.to |= (unsigned long long)map_at(b.to, m) << (4 * i);
-        r.bad |= ((b.bad >> m) & 1u) << i;
-    }
-    return r;
-}
-
-struct SeqShared {
-    unsigned long long to[kSeqLevels][kSeqThreads];
-    uint16_t bad[kSeqLevels][kSeqThreads];
-    int entry[BORN_MAX_BEAMS];   // beam at the bottom of the chunk in which the hypothesis ends, -1 = bad
-    int end[BORN_MAX_BEAMS], first[BORN_MAX_BEAMS];
-};
+constexpr int kSeqThreads = 1024;
+constexpr int kSeqChunks = kSeqThreads / 16;
+constexpr uint32_t kNoLink = 0x80u;
 
 __global__ void __launch_bounds__(kSeqThreads) sequences_kernel(const SequencesArgs A) {
-    extern __shared__ unsigned long long step_to[];  // [T], then step_bad [T] (16 bits each)
-    __shared__ SeqShared sh;
-    uint16_t* step_bad = reinterpret_cast<uint16_t*>(step_to + A.T);
-    const int n = blockIdx.x, tid = threadIdx.x;
-    const int K = A.K, T = A.T, H = A.H;
+    extern __shared__ __align__(16) int32_t token_at[];  // [tile][width] tokens; then parents and beams, a byte each
+    __shared__ int8_t map[kSeqChunks][BORN_MAX_BEAMS];    // beam of a chunk's last step -> beam below its first
+    __shared__ int8_t entry[kSeqChunks][BORN_MAX_BEAMS];  // beam of hypothesis h at a chunk's last step
+    __shared__ int8_t low[BORN_MAX_BEAMS];                // ... below the chunk in which it ends
+    __shared__ int8_t carry[BORN_MAX_BEAMS];              // ... at the last step of the tile that comes next
+    __shared__ int ends[BORN_MAX_BEAMS];
+    __shared__ int32_t last[BORN_MAX_BEAMS];
+    const int n = blockIdx.x, tid = threadIdx.x, chunk = tid >> 4, l = tid & 15;
+    const int K = A.K, T = A.T, H = A.H, shift = A.shift, W = 1 << shift;
+    uint8_t* link = reinterpret_cast<uint8_t*>(token_at + A.tile * W);  // a step's parents; kNoLink: none
+    uint8_t* beam = link + A.tile * W;                                  // beams of the hypotheses at a step
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int32_t* parents = A.parents + (int64_t)n * K;
     const int32_t* tokens = A.tokens + (int64_t)n * K;
-    const int C = (T + kSeqThreads - 1) / kSeqThreads;  // steps of a thread
-
-    // Map of step t: beam of step t -> beam of step t - 1 (there is none before step 0: the identity).
-    for (int t = tid; t < T; t += kSeqThreads) {
-        unsigned long long to = t ? 0 : kIdentity;
-        uint32_t bad = 0;
-        for (int b = 0; b < K && t; ++b) {
-            const int p = parents[t * A.table_stride + b];
-            if (p < 0 || p >= K) bad |= 1u << b;
-            else to |= (unsigned long long)p << (4 * b);
+    int32_t* out = A.out_tokens + (int64_t)n * H * A.out_stride;
+    // hypothesis l: its last step (-1: empty) and the beam before it
+    int e = -1, first = 0;
+    if (l < H) {
+        e = A.end_step[(int64_t)n * H + l];
+        first = A.end_parent[(int64_t)n * H + l];
+        if (tid < 16) last[l] = A.end_token[(int64_t)n * H + l];
+    }
+    if (e < 0 || e >= T || first < 0 || first >= K) e = -1;
+    if (tid < 16) {
+        ends[l] = e;
+        carry[l] = 0;
+    }
+    for (int tile = (T - 1) / A.tile; tile >= 0; --tile) {
+        const int base = tile * A.tile, steps = min(A.tile, T - base);
+        const int C = (steps + kSeqChunks - 1) / kSeqChunks, lo = chunk * C, hi = min(steps, lo + C);
+        // ---- the tables' rows; before step 0 a beam's parent is itself
+        for (int i0 = tid; i0 < steps << shift; i0 += 8 * kSeqThreads) {
+            int32_t p[8], v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u * kSeqThreads, t = i >> shift, b = i & (W - 1);
+                const bool ok = t < steps && b < K;
+                p[u] = ok ? parents[(int64_t)(base + t) * A.table_stride + b] : 0;
+                v[u] = ok ? tokens[(int64_t)(base + t) * A.table_stride + b] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u * kSeqThreads, t = i >> shift, b = i & (W - 1);
+                if (t >= steps) break;
+                link[i] = (uint8_t)(base + t == 0 ? b : p[u] < 0 || p[u] >= K ? kNoLink : p[u]);
+                token_at[i] = v[u];
+            }
         }
-        step_to[t] = to;
-        step_bad[t] = (uint16_t)bad;
-    }
-    __syncthreads();
-    // Map of chunk c: beam of its last step -> beam of the step before its first.
-    {
-        BeamMap m = {kIdentity, 0};
-        for (int t = min(T, (tid + 1) * C) - 1; t >= tid * C; --t) m = compose(m, BeamMap{step_to[t], step_bad[t]});
-        sh.to[0][tid] = m.to;
-        sh.bad[0][tid] = (uint16_t)m.bad;
-    }
-    __syncthreads();
-    // level l: the maps of 2^l chunks, the last of which is c
-    for (int l = 1; l < kSeqLevels; ++l) {
-        const int d = 1 << (l - 1);
-        if (tid >= 2 * d - 1) {
-            const BeamMap m = compose(BeamMap{sh.to[l - 1][tid], sh.bad[l - 1][tid]}, BeamMap{sh.to[l - 1][tid - d], sh.bad[l - 1][tid - d]});
-            sh.to[l][tid] = m.to;
-            sh.bad[l][tid] = (uint16_t)m.bad;
+        __syncthreads();
+        // ---- the chunks' maps, and the hypotheses from their end to the bottom of its chunk
+        const int at = e - 1 - base;  // the hypothesis joins here
+        const bool joins = e > 0 && at >= 0 && at < steps;
+        {
+            uint32_t r = l & (W - 1), b = 0, bad_r = 0, bad_b = 0;
+            const uint8_t* row = link + (hi << shift);
+            for (int t = hi - 1; t >= lo; --t) {
+                row -= W;
+                if (t == at) {
+                    b = first;
+                    bad_b = 0;
+                }
+                r = row[r];
+                b = row[b];
+                bad_r |= r;
+                bad_b |= b;
+                r &= 15u;
+                b &= 15u;
+            }
+            map[chunk][l] = (int8_t)(bad_r & kNoLink ? -1 : (int)r);
+            if (joins && at / C == chunk) low[l] = (int8_t)(bad_b & kNoLink ? -1 : (int)b);
+        }
+        __syncthreads();
+        // ---- from chunk to chunk; a missing link empties the hypothesis
+        if (tid < 16) {
+            int c = -1, b = 0;
+            if (joins) {
+                c = at / C - 1;
+                b = low[l];
+            } else if (e - 1 >= base + steps) {
+                c = (steps - 1) / C;
+                b = carry[l];
+            }
+            const bool walks = joins || c >= 0;
+            for (; c >= 0 && b >= 0; --c) {
+                entry[c][l] = (int8_t)b;
+                b = map[c][b];
+            }
+            if (walks) {
+                carry[l] = (int8_t)max(b, 0);
+                if (b < 0) ends[l] = e = -2;  // (written before it was known: see below)
+            }
+        }
+        __syncthreads();
+        if (ends[l] < 0) e = ends[l];
+        // ---- the hypotheses' beams, step by step
+        {
+            uint32_t b = e - 1 >= base + hi ? entry[chunk][l] : 0;
+            int i = hi << shift;
+            for (int t = hi - 1; t >= lo; --t) {
+                i -= W;
+                if (t == at) b = first;
+                if (l < H) beam[i + l] = (uint8_t)b;
+                b = link[i + b] & 15u;
+            }
+        }
+        __syncthreads();
+        // ---- the tokens
+        for (int h = 0; h < H; ++h) {
+            const int eh = ends[h] - base;
+            for (int t = tid; t < steps; t += kSeqThreads)
+                out[h * A.out_stride + base + t] = t < eh ? token_at[(t << shift) + beam[(t << shift) + h]] : t == eh ? last[h] : A.pad;
         }
         __syncthreads();
     }
-    // The hypotheses: from their end to the bottom of its chunk, then all the way to see that no link is missing.
-    if (tid < H) {
-        int e = A.end_step[(int64_t)n * H + tid];
-        const int p = A.end_parent[(int64_t)n * H + tid];
-        if (e < 0 || e >= T || p < 0 || p >= K) e = -1;
-        int b = p, low = -1;
-        if (e >= 0) {
-            int t = e - 1;
-            const int c = t >= 0 ? t / C : 0;
-            for (; t >= c * C && b >= 0; --t) b = (step_bad[t] >> b) & 1 ? -1 : map_at(step_to[t], b);
-            low = b;
-            int at = c - 1;
-            for (int l = kSeqLevels - 1; l >= 0 && b >= 0; --l) {
-                if (at + 1 < (1 << l)) continue;
-                b = (sh.bad[l][at] >> b) & 1 ? -1 : map_at(sh.to[l][at], b);
-                at -= 1 << l;
-            }
-            if (b < 0) e = -1;
-        }
-        sh.end[tid] = e;
-        sh.first[tid] = p;
-        sh.entry[tid] = low;
-        A.out_lens[(int64_t)n * H + tid] = e + 1;
-    }
-    __syncthreads();
-    const int lo = tid * C, hi = min(T, lo + C);
-    for (int h = 0; h < H; ++h) {
-        const int e = sh.end[h];
-        int32_t* out = A.out_tokens + ((int64_t)n * H + h) * A.out_stride;
-        int b = -1;
-        if (e - 1 >= lo && e - 1 < hi) b = sh.first[h];
-        else if (e - 1 >= hi) {
-            b = sh.entry[h];
-            int at = (e - 1) / C - 1;
-            for (int l = kSeqLevels - 1; l >= 0; --l) {
-                if (at - tid < (1 << l)) continue;
-                b = map_at(sh.to[l][at], b);
-                at -= 1 << l;
-            }
-        }
-        for (int t = hi - 1; t >= lo; --t) {
-            int32_t v = A.pad;
-            if (t == e) v = A.end_token[(int64_t)n * H + h];
-            else if (t < e) {
-                v = tokens[t * A.table_stride + b];
-                b = map_at(step_to[t], b);
-            }
-            out[t] = v;
-        }
-    }
+    if (tid < H) A.out_lens[(int64_t)n * H + tid] = max(ends[tid], -1) + 1;
+    // hypotheses whose missing link lay in an earlier tile than tokens already written
+    if (T > A.tile)
+        for (int h = 0; h < H; ++h)
+            if (ends[h] == -2)
+                for (int t = tid; t < T; t += kSeqThreads) out[h * A.out_stride + t] = A.pad;
 }
 
 }  // namespace born

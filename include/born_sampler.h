@@ -73,7 +73,6 @@ extern "C" {
 #define BORN_MAX_BEAMS 16          /* beams of a group */
 #define BORN_MAX_STOPS 8           /* stop tokens */
 #define BORN_MAX_REORDER 128       /* buffers of one born_beam_reorder call */
-#define BORN_MAX_STEPS 16384       /* steps of the tables that born_beam_sequences reads */
 
 #define BORN_DTYPE_F32 0
 #define BORN_DTYPE_BF16 1

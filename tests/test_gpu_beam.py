@@ -423,7 +423,7 @@ def test_reorder_past_32_bits(s):
 
 
 # ---- sequences ---------------------------------------------------------------------------------
-@pytest.mark.parametrize("N,K,T,H", [(1, 1, 1, 1), (2, 4, 2, 4), (3, 16, 255, 16), (1, 5, 256, 3), (2, 8, 257, 8), (4, 3, 1000, 5), (1, 16, 16384, 2)])
+@pytest.mark.parametrize("N,K,T,H", [(1, 1, 1, 1), (2, 4, 2, 4), (3, 16, 255, 16), (1, 5, 256, 3), (2, 8, 257, 8), (4, 3, 1000, 5), (1, 16, 16384, 2), (1, 2, 70001, 2), (2, 4, 512, 4), (2, 4, 513, 4)])
 @pytest.mark.parametrize("broken", [False, True])
 def test_sequences(s, N, K, T, H, broken):
     rng = np.random.default_rng(T)
@@ -616,6 +616,5 @@ def test_refusals(s):
     bad(*inv, s.beam_sequences, t, t, e, e, e[:1], K)
     bad(*inv, s.beam_sequences, t, t, e[:1], e, e, K)
     bad(*inv, s.beam_sequences, t.long(), t, e, e, e, K)
-    bad(*uns, s.beam_sequences, torch.zeros((16385, 8), **i32), torch.zeros((16385, 8), **i32), e, e, e, K)
     e17 = torch.zeros((2, 17), **i32)
     bad(*uns, s.beam_sequences, t, t, e17, e17, e17, K)
