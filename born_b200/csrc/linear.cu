@@ -30,38 +30,81 @@ static bool make_map(CUtensorMap* map, const void* p, int rows, int K, int64_t s
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename O, int kCols, bool kPair>
+static cudaError_t raise_limit() {
+    return cudaFuncSetAttribute(linear_kernel<O, kCols, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem);
+}
+template <typename O>
+static cudaError_t raise_limits() {
+    cudaError_t e;
+    if ((e = raise_limit<O, 16, false>()) != cudaSuccess || (e = raise_limit<O, 32, false>()) != cudaSuccess) return e;
+    if ((e = raise_limit<O, 64, false>()) != cudaSuccess || (e = raise_limit<O, 128, false>()) != cudaSuccess) return e;
+    if ((e = raise_limit<O, 64, true>()) != cudaSuccess) return e;
+    return raise_limit<O, 128, true>();
+}
 cudaError_t linear_attrs() {
-    cudaError_t e = cudaFuncSetAttribute(linear_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem);
-    return e;
+    const cudaError_t e = raise_limits<float>();
+    return e != cudaSuccess ? e : raise_limits<__nv_bfloat16>();
+}
+
+template <typename O, int kCols, bool kPair>
+static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, unsigned grid, cudaStream_t st) {
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = kPair ? 2 : 1;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(kLinThreads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)P.stages * P.stage_bytes + 1024;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = kPair ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair>, w, x, P);
+}
+template <typename O>
+static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, bool pair, unsigned grid, cudaStream_t st) {
+    const int cols = P.cols > 16 ? P.cols / 2 : 16;
+    if (pair) return cols <= 64 ? launch<O, 64, true>(w, x, P, grid, st) : launch<O, 128, true>(w, x, P, grid, st);
+    if (cols <= 16) return launch<O, 16, false>(w, x, P, grid, st);
+    if (cols <= 32) return launch<O, 32, false>(w, x, P, grid, st);
+    return cols <= 64 ? launch<O, 64, false>(w, x, P, grid, st) : launch<O, 128, false>(w, x, P, grid, st);
 }
 
 cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStream_t st) {
     LinearParams P;
     memset(&P, 0, sizeof P);
     P.M = A.M; P.K = A.K; P.V = A.V;
-    // as few column tiles as hold the rows, of equal widths
-    P.m_tiles = (A.M + kLinMaxCols - 1) / kLinMaxCols;
-    P.cols = ((A.M + P.m_tiles - 1) / P.m_tiles + 15) / 16 * 16;
-    P.m_tiles = (A.M + P.cols - 1) / P.cols;
+    // as few column tiles as hold the rows, more where that leaves most of the GPU idle, of equal widths
     P.v_tiles = (A.V + kLinRows - 1) / kLinRows;
-    P.stage_bytes = (kLinRows + P.cols) * kLinK * 2;  // (16 rows of a slice are 2 KB: atoms stay on 1024 bytes)
+    int most = kLinMaxCols;
+    while (most > 64 && (int64_t)P.v_tiles * ((A.M + most - 1) / most) * 2 <= num_sms && A.M > most / 2) most /= 2;
+    P.m_tiles = (A.M + most - 1) / most;
+    const int unit = A.M <= 16 ? 16 : 32;  // (a multiple of 16 for either half of the epilogue)
+    P.cols = ((A.M + P.m_tiles - 1) / P.m_tiles + unit - 1) / unit * unit;
+    P.m_tiles = (A.M + P.cols - 1) / P.cols;
+    // A pair from 65 columns on: below that the batch's slices are a third of the bytes at most
+    const bool pair = P.cols > 64 && A.V > kLinRows;
+    if (pair) P.v_tiles = (A.V + 2 * kLinRows - 1) / (2 * kLinRows);
+    const int x_rows = pair ? P.cols / 2 : P.cols;  // of the batch in a CTA
+    P.stage_bytes = (kLinRows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
     P.stages = (kLinSmem - 1024) / P.stage_bytes;
     if (P.stages > kLinMaxStages) P.stages = kLinMaxStages;
     P.tmem_cols = 32;
     while (P.tmem_cols < 2 * P.cols) P.tmem_cols *= 2;
-    P.activation = A.activation; P.scale = A.scale;
+    P.activation = A.activation; P.scale = A.scale; P.inv_scale = 1.0f / A.scale;
     P.bias = A.bias; P.residual = A.residual; P.out = A.out;
     P.residual_stride = A.residual_stride; P.out_stride = A.out_stride;
     P.dev_error = A.dev_error; P.timeout_ns = A.timeout_ns;
     CUtensorMap w, x;
-    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, P.cols)) return cudaErrorInvalidValue;
-    const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles;
-    const unsigned grid = (unsigned)(tiles < num_sms ? tiles : num_sms);
-    const size_t smem = (size_t)P.stages * P.stage_bytes + 1024;
-    if (dtype == BORN_DTYPE_F32) linear_kernel<float><<<grid, kLinThreads, smem, st>>>(w, x, P);
-    else linear_kernel<__nv_bfloat16><<<grid, kLinThreads, smem, st>>>(w, x, P);
-    return cudaGetLastError();
+    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
+    const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles, room = pair ? num_sms / 2 : num_sms;
+    const unsigned grid = (unsigned)(tiles < room ? tiles : room) * (pair ? 2u : 1u);
+    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, x, P, pair, grid, st);
+    return launch_as<__nv_bfloat16>(w, x, P, pair, grid, st);
 }
 
 }  // namespace born

@@ -2,10 +2,18 @@
 //
 // A decode batch has few rows and a vocabulary many, so the weights take the tile's 128 rows and the
 // batch its columns (16 to 256): D[128 v][n m] = W[128][K] X[n][K]^T, both operands K-major as they lie in
-// memory.  One CTA per SM walks over tiles; a warp fills a ring of 64-element slices of both operands by
+// memory.  A CTA per SM walks over tiles; a thread fills a ring of 64-element slices of both operands by
 // TMA (128-byte swizzle), a thread issues the tcgen05 products into one of two accumulators in tensor
-// memory, four warps empty the other one: a lane holds one v, so that a column of 32 lanes is a
+// memory, eight warps empty the other one: a lane holds one v, so that a column of 32 lanes is a
 // contiguous piece of an output row.
+//
+// Two CTAs share a tile of 256 v from 65 columns on (kPair): each holds its own 128 rows of weights and half
+// of the batch's rows, which the other one's tensor core reads too.  One CTA alone reads the batch's slice
+// for every 128 rows of weights, and 256 columns of it twice the weights' bytes: out of L2, 256 rows of hidden
+// 4096 over 128256 features took 330 us with that.
+//
+// The tensor core cuts partial sums off rather than rounding them, once per 16 products, which adds up: 4.3e-6 of
+// the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded.
 //
 // What bounds it: up to some 200 rows the bytes of the weights, beyond that the tensor pipe.
 #pragma once
@@ -20,20 +28,21 @@
 
 namespace born {
 
-constexpr int kLinRows = 128;      // v of a tile
+constexpr int kLinRows = 128;      // v of a CTA's tile
 constexpr int kLinK = 64;          // elements of a slice: 128 bytes, one swizzle atom
+constexpr int kLinChunk = 8;       // slices that the tensor core sums
 constexpr int kLinMaxCols = 256;   // m of a tile
 constexpr int kLinMaxStages = 12;
-constexpr int kLinThreads = 256;   // warps: 0 TMA, 1 products, 2 tensor memory, 3 idle, 4..7 epilogue
+constexpr int kLinThreads = 384;   // warps: 0 TMA, 1 products, 2 tensor memory, 3 idle, 4..11 epilogue
 constexpr int kLinSmem = 220 * 1024;
 
 struct LinearParams {
     int M, K, V;
-    int cols;          // m of a tile, a multiple of 16
+    int cols;          // m of a tile
     int v_tiles, m_tiles;
-    int stages, stage_bytes, tmem_cols;
+    int stages, stage_bytes, tmem_cols;  // of a CTA
     int activation;
-    float scale;
+    float scale, inv_scale;
     const float* bias;
     const void* residual;
     void* out;
@@ -66,7 +75,6 @@ __device__ __forceinline__ bool lin_wait(LinearShared& sh, uint64_t* bar, uint32
     sh.failed = 1;
     return false;
 }
-
 // Bounded wait whatever happened elsewhere.
 __device__ __forceinline__ void lin_settle(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
     const unsigned long long t0 = global_timer_ns();
@@ -78,39 +86,66 @@ __device__ __forceinline__ void lin_settle(uint32_t bar, uint32_t parity, unsign
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+// bar: of the pair's first CTA in kPair, whose bytes both CTAs' copies count towards
+template <bool kPair>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-                 "l"(map), "r"(x), "r"(y), "r"(bar)
-                 : "memory");
+    if constexpr (kPair)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(bar & 0xFEFFFFFFu)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
 }
+template <bool kPair>
 __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if constexpr (kPair)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
+// An arrival, once the products issued so far are done, at the barrier (of both CTAs in kPair).
+template <bool kPair>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if constexpr (kPair)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+// An arrival at the barrier of the pair's first CTA.
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
 }
-__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
-    uint32_t r[16];
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Adds 16 columns of the accumulator to v, or replaces it by them.
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
           "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-__device__ __forceinline__ void activate(int activation, float scale, float (&v)[16]) {
-    switch (activation) {
+__device__ __forceinline__ void activate(const LinearParams& P, float* v) {
+    switch (P.activation) {
         case BORN_ACT_RELU:
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
@@ -121,7 +156,7 @@ __device__ __forceinline__ void activate(int activation, float scale, float (&v)
             break;
         case BORN_ACT_TANH:
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = scale * tanhf(v[i] / scale);
+            for (int i = 0; i < 16; ++i) v[i] = P.scale * tanhf(v[i] * P.inv_scale);
             break;
         case BORN_ACT_GELU:
 #pragma unroll
@@ -140,15 +175,21 @@ __device__ __forceinline__ float load_out(const __nv_bfloat16* p) { return __bfl
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename O>
+// kCols: columns of the tile that a thread of the epilogue holds at most (the two groups of four warps take half
+// of the tile's columns each, or the first one all 16).
+template <typename O, int kCols, bool kPair>
 __global__ void __launch_bounds__(kLinThreads, 1)
-linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const LinearParams P) {
+linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ LinearParams P) {
     extern __shared__ uint8_t raw[];
     __shared__ LinearShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;  // swizzle atoms start on 1024 bytes
+    const int rank = kPair ? (int)(blockIdx.x & 1u) : 0;     // in the pair
+    const int first = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int tiles = P.v_tiles * P.m_tiles;
     const int slices = (P.K + kLinK - 1) / kLinK;
+    const int groups = P.cols > 16 ? 2 : 1;                  // of warps that take part in the epilogue
+    constexpr int kTileRows = kPair ? 2 * kLinRows : kLinRows;
     if (tid == 0) {
         for (int i = 0; i < P.stages; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -156,127 +197,178 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.acc_full[i], 1);
-            mbar_init(&sh.acc_empty[i], 4);
+            mbar_init(&sh.acc_empty[i], (uint32_t)(4 * groups * (kPair ? 2 : 1)));
         }
         mbar_init(&sh.drained, 1);
         sh.failed = 0;
         mbar_fence_init();
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(P.tmem_cols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(P.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(P.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (kPair) cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sh.tmem;
     const uint32_t x_at = kLinRows * kLinK * 2;  // the batch's slice behind the weights' one
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == 0 && lane == 0) {
-        // ---- producer
+        // ---- producer: this CTA's rows of weights, its share of the batch's
         int stage = 0;
         uint32_t phase = 0;
         long long issued = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const int v0 = t / P.m_tiles * kLinRows, m0 = t % P.m_tiles * P.cols;
+        for (int t = first; t < tiles && ok; t += step) {
+            const int v0 = t / P.m_tiles * kTileRows + rank * kLinRows;
+            const int m0 = t % P.m_tiles * P.cols + (kPair ? rank * (P.cols / 2) : 0);
             for (int k = 0; k < slices; ++k) {
                 if (!lin_wait(sh, &sh.empty[stage], phase ^ 1u, P.timeout_ns)) {
                     ok = false;
                     break;
                 }
                 const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * P.stage_bytes);
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(P.stage_bytes) : "memory");
-                tma_load_2d(at, &wmap, k * kLinK, v0, bar);
-                tma_load_2d(at + x_at, &xmap, k * kLinK, m0, bar);
+                if (rank == 0)
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(P.stage_bytes * (kPair ? 2 : 1)) : "memory");
+                tma_load_2d<kPair>(at, &wmap, k * kLinK, v0, bar);
+                tma_load_2d<kPair>(at + x_at, &xmap, k * kLinK, m0, bar);
                 ++issued;
                 if (++stage == P.stages) { stage = 0; phase ^= 1u; }
             }
         }
-        // the copies in flight land before the CTA ends (bounded, whatever happened to the others)
-        const int last = issued < P.stages ? (int)issued : P.stages;
+        // the copies in flight land before the CTA ends (bounded, whatever happened to the others; the first CTA's
+        // barriers count the second one's too, and neither ends before the other)
+        const int last = rank != 0 ? 0 : issued < P.stages ? (int)issued : P.stages;
         for (int i = 0; i < last; ++i) {
             if (--stage < 0) { stage = P.stages - 1; phase ^= 1u; }
             lin_settle(smem_u32(&sh.full[stage]), phase, P.timeout_ns);
         }
-    } else if (warp == 1 && lane == 0) {
-        // ---- products: D fp32, A and B bf16, both K-major, N = cols, M = 128
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(P.cols >> 3) << 17) | ((uint32_t)(kLinRows >> 4) << 24);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // ---- products: D fp32, A and B bf16, both K-major
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(P.cols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
         int stage = 0, n = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
-            const int acc = n & 1;
-            if (!lin_wait(sh, &sh.acc_empty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, P.timeout_ns)) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t d = tmem + (uint32_t)(acc * P.cols);
-            for (int k = 0; k < slices; ++k) {
-                if (!lin_wait(sh, &sh.full[stage], phase, P.timeout_ns)) {
+        for (int t = first; t < tiles && ok; t += step) {
+            for (int k0 = 0; k0 < slices && ok; k0 += kLinChunk, ++n) {
+                const int acc = n & 1;
+                if (!lin_wait(sh, &sh.acc_empty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, P.timeout_ns)) {
                     ok = false;
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t at = ring + (uint32_t)(stage * P.stage_bytes);
-                const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
+                const uint32_t d = tmem + (uint32_t)(acc * P.cols);
+                const int k1 = min(slices, k0 + kLinChunk);
+                for (int k = k0; k < k1; ++k) {
+                    if (!lin_wait(sh, &sh.full[stage], phase, P.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = ring + (uint32_t)(stage * P.stage_bytes);
+                    const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
 #pragma unroll
-                for (int i = 0; i < kLinK / 16; ++i) mma_bf16(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)(k | i));
-                mma_commit(&sh.empty[stage]);
-                if (++stage == P.stages) { stage = 0; phase ^= 1u; }
+                    for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
+                    mma_commit<kPair>(&sh.empty[stage]);
+                    if (++stage == P.stages) { stage = 0; phase ^= 1u; }
+                }
+                if (ok) mma_commit<kPair>(&sh.acc_full[acc]);
             }
-            if (ok) mma_commit(&sh.acc_full[acc]);
         }
         // tensor memory is given back only after the last product (bounded, like the copies)
-        mma_commit(&sh.drained);
+        mma_commit<kPair>(&sh.drained);
         lin_settle(smem_u32(&sh.drained), 0, P.timeout_ns);
-    } else if (warp >= 4) {
+    } else if (warp >= 4 && (warp - 4) >> 2 < groups) {
         // ---- epilogue
+        const int half = P.cols / groups, c0 = ((warp - 4) >> 2) * half, quad = warp & 3;
+        const uint32_t d0 = tmem + ((uint32_t)quad << 21) + (uint32_t)c0;
         int n = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
-            const int acc = n & 1;
-            int ok = 1;
-            if (lane == 0) ok = lin_wait(sh, &sh.acc_full[acc], (uint32_t)(n >> 1) & 1u, P.timeout_ns);
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok) break;
-            // (every lane observes the phase itself before it reads what the products wrote)
-            ring_try(smem_u32(&sh.acc_full[acc]), (uint32_t)(n >> 1) & 1u);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int v = t / P.m_tiles * kLinRows + (warp - 4) * 32 + lane, m0 = t % P.m_tiles * P.cols;
-            const int count = min(P.cols, P.M - m0);
-            const uint32_t d = tmem + ((uint32_t)(warp - 4) << 21) + (uint32_t)(acc * P.cols);
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+            const int v = t / P.m_tiles * kTileRows + rank * kLinRows + quad * 32 + lane, m0 = t % P.m_tiles * P.cols + c0;
+            const int count = min(half, P.M - m0);  // (none for a group whose columns lie behind the batch)
             const bool in = v < P.V;
             const float bias = P.bias && in ? P.bias[v] : 0.0f;
+            float y[kCols];
+            for (int k0 = 0; k0 < slices; k0 += kLinChunk, ++n) {
+                const int acc = n & 1;
+                int got = 1;
+                if (lane == 0) got = lin_wait(sh, &sh.acc_full[acc], (uint32_t)(n >> 1) & 1u, P.timeout_ns);
+                ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+                if (!ok) break;
+                // (every lane observes the phase itself before it reads what the products wrote)
+                ring_try(smem_u32(&sh.acc_full[acc]), (uint32_t)(n >> 1) & 1u);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = d0 + (uint32_t)(acc * P.cols);
+#pragma unroll
+                for (int c = 0; c < kCols; c += 16) {
+                    if (c >= half) break;
+                    uint32_t r[16];
+                    tmem_load16(d + (uint32_t)c, r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (k0 == 0) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[c + i] = __uint_as_float(r[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[c + i] += __uint_as_float(r[i]);
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (kPair) arrive_first(&sh.acc_empty[acc]);
+                    else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.acc_empty[acc])) : "memory");
+                }
+            }
+            if (!ok) break;
             O* out = reinterpret_cast<O*>(P.out) + (int64_t)m0 * P.out_stride + v;
             const O* res = reinterpret_cast<const O*>(P.residual) + (int64_t)m0 * P.residual_stride + v;
-            for (int c = 0; c < count; c += 16) {
-                float y[16], r[16];
-                tmem_load16(d + (uint32_t)c, y);
-                if (P.residual) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) r[i] = in && c + i < count ? load_out(res + (int64_t)(c + i) * P.residual_stride) : 0.0f;
-                }
+            for (int c = 0; c < kCols; c += 16) {
+                if (c >= count) break;
                 if (P.bias) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) y[i] += bias;
+                    for (int i = 0; i < 16; ++i) y[c + i] += bias;
                 }
-                activate(P.activation, P.scale, y);
+                activate(P, y + c);
+                // (an address at a time: 128 of them would not fit the registers)
                 if (P.residual) {
+                    float r[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) y[i] += r[i];
+                    for (int i = 0; i < 16; ++i) {
+                        r[i] = in && c + i < count ? load_out(res) : 0.0f;
+                        res += P.residual_stride;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[c + i] += r[i];
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (in && c + i < count) store_out(out + (int64_t)(c + i) * P.out_stride, y[i]);
+                for (int i = 0; i < 16; ++i) {
+                    if (in && c + i < count) store_out(out, y[c + i]);
+                    out += P.out_stride;
+                }
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.acc_empty[acc]);
         }
     }
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (kPair) cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (tid == 0 && sh.failed) atomicExch(P.dev_error, BORN_ERR_DEVICE_TIMEOUT);
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols) : "memory");
+    if (warp == 2) {
+        if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols) : "memory");
+    }
 }
 
 }  // namespace born
