@@ -42,6 +42,8 @@ static cudaError_t raise_limits() {
     if ((e = raise_limit<O, 64, true>()) != cudaSuccess) return e;
     return raise_limit<O, 128, true>();
 }
+int64_t linear_scratch_bytes(int num_sms) { return (int64_t)num_sms * kLinSplitCols * kLinRows * 4; }
+int linear_tickets(int num_sms) { return num_sms; }
 cudaError_t linear_attrs() {
     const cudaError_t e = raise_limits<float>();
     return e != cudaSuccess ? e : raise_limits<__nv_bfloat16>();
@@ -78,10 +80,9 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStrea
     LinearParams P;
     memset(&P, 0, sizeof P);
     P.M = A.M; P.K = A.K; P.V = A.V;
-    // as few column tiles as hold the rows, more where that leaves most of the GPU idle, of equal widths
     P.v_tiles = (A.V + kLinRows - 1) / kLinRows;
-    int most = kLinMaxCols;
-    while (most > 64 && (int64_t)P.v_tiles * ((A.M + most - 1) / most) * 2 <= num_sms && A.M > most / 2) most /= 2;
+    // as few column tiles as hold the rows, of equal widths; 128 columns at most where the tiles are few
+    const int most = (int64_t)P.v_tiles * ((A.M + kLinMaxCols - 1) / kLinMaxCols) * 2 <= num_sms ? kLinSplitCols : kLinMaxCols;
     P.m_tiles = (A.M + most - 1) / most;
     const int unit = A.M <= 16 ? 16 : 32;  // (a multiple of 16 for either half of the epilogue)
     P.cols = ((A.M + P.m_tiles - 1) / P.m_tiles + unit - 1) / unit * unit;
@@ -89,6 +90,17 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStrea
     // A pair from 65 columns on: below that the batch's slices are a third of the bytes at most
     const bool pair = P.cols > 64 && A.V > kLinRows;
     if (pair) P.v_tiles = (A.V + 2 * kLinRows - 1) / (2 * kLinRows);
+    // K is shared out while CTAs are left, in parts of four slices at least; adding up the parts costs the one that
+    // does it their bytes, so wide tiles get few
+    const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles, room = pair ? num_sms / 2 : num_sms;
+    const int slices = (A.K + kLinK - 1) / kLinK;
+    int64_t splits = room / tiles;
+    if (splits > slices / 4) splits = slices / 4;
+    if (splits > 1024 / P.cols) splits = 1024 / P.cols;
+    if (splits < 1 || P.cols > kLinSplitCols) splits = 1;
+    P.part = (int)((slices + splits - 1) / splits);
+    P.splits = (slices + P.part - 1) / P.part;
+    P.partial = A.partial; P.tickets = A.tickets;
     const int x_rows = pair ? P.cols / 2 : P.cols;  // of the batch in a CTA
     P.stage_bytes = (kLinRows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
     P.stages = (kLinSmem - 1024) / P.stage_bytes;
@@ -101,8 +113,8 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStrea
     P.dev_error = A.dev_error; P.timeout_ns = A.timeout_ns;
     CUtensorMap w, x;
     if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
-    const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles, room = pair ? num_sms / 2 : num_sms;
-    const unsigned grid = (unsigned)(tiles < room ? tiles : room) * (pair ? 2u : 1u);
+    const int64_t units = tiles * P.splits;
+    const unsigned grid = (unsigned)(units < room ? units : room) * (pair ? 2u : 1u);
     if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, x, P, pair, grid, st);
     return launch_as<__nv_bfloat16>(w, x, P, pair, grid, st);
 }

@@ -15,6 +15,11 @@
 // The tensor core cuts partial sums off rather than rounding them, once per 16 products, which adds up: 4.3e-6 of
 // the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded.
 //
+// Where the tiles are too few for the GPU, several CTAs (or pairs) share one, each with a part of K (splits).  They
+// leave their sums in scratch; the one that draws the tile's last ticket adds them up, in the order of the parts, and
+// finishes the tile.  No CTA waits for another one.  8192 x 1024 weights for one row: 45 us on the eight SMs that
+// have a tile, 12 us split.
+//
 // What bounds it: up to some 200 rows the bytes of the weights, beyond that the tensor pipe.
 #pragma once
 #include <cuda.h>
@@ -32,6 +37,7 @@ constexpr int kLinRows = 128;      // v of a CTA's tile
 constexpr int kLinK = 64;          // elements of a slice: 128 bytes, one swizzle atom
 constexpr int kLinChunk = 8;       // slices that the tensor core sums
 constexpr int kLinMaxCols = 256;   // m of a tile
+constexpr int kLinSplitCols = 128; // ... where K is shared out (the scratch is sized for it)
 constexpr int kLinMaxStages = 12;
 constexpr int kLinThreads = 384;   // warps: 0 TMA, 1 products, 2 tensor memory, 3 idle, 4..11 epilogue
 constexpr int kLinSmem = 220 * 1024;
@@ -40,6 +46,9 @@ struct LinearParams {
     int M, K, V;
     int cols;          // m of a tile
     int v_tiles, m_tiles;
+    int splits, part;  // CTAs (pairs) of a tile; slices of each
+    float* partial;    // [tile of a CTA][split][cols][kLinRows]
+    uint32_t* tickets; // [tile of a CTA]
     int stages, stage_bytes, tmem_cols;  // of a CTA
     int activation;
     float scale, inv_scale;
@@ -55,6 +64,7 @@ struct LinearShared {
     uint64_t full[kLinMaxStages], empty[kLinMaxStages];
     uint64_t acc_full[2], acc_empty[2], drained;
     uint32_t tmem;
+    int last;
     volatile int failed;
 };
 
@@ -131,6 +141,19 @@ __device__ __forceinline__ void arrive_first(uint64_t* bar) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
 }
+// Barrier of the epilogue's threads: whether any of them says so.
+__device__ __forceinline__ bool epilogue_any(bool pred, int threads) {
+    int r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.s32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, %2, p;\n\t"
+        "selp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((int)pred), "r"(threads)
+        : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -186,8 +209,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;  // swizzle atoms start on 1024 bytes
     const int rank = kPair ? (int)(blockIdx.x & 1u) : 0;     // in the pair
     const int first = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
-    const int tiles = P.v_tiles * P.m_tiles;
-    const int slices = (P.K + kLinK - 1) / kLinK;
+    const int units = P.v_tiles * P.m_tiles * P.splits;      // tiles, times the parts of K
+    const int all_slices = (P.K + kLinK - 1) / kLinK;
     const int groups = P.cols > 16 ? 2 : 1;                  // of warps that take part in the epilogue
     constexpr int kTileRows = kPair ? 2 * kLinRows : kLinRows;
     if (tid == 0) {
@@ -227,7 +250,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         uint32_t phase = 0;
         long long issued = 0;
         bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
+        for (int u = first; u < units && ok; u += step) {
+            const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
             const int v0 = t / P.m_tiles * kTileRows + rank * kLinRows;
             const int m0 = t % P.m_tiles * P.cols + (kPair ? rank * (P.cols / 2) : 0);
             for (int k = 0; k < slices; ++k) {
@@ -238,8 +262,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * P.stage_bytes);
                 if (rank == 0)
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(P.stage_bytes * (kPair ? 2 : 1)) : "memory");
-                tma_load_2d<kPair>(at, &wmap, k * kLinK, v0, bar);
-                tma_load_2d<kPair>(at + x_at, &xmap, k * kLinK, m0, bar);
+                tma_load_2d<kPair>(at, &wmap, (s0 + k) * kLinK, v0, bar);
+                tma_load_2d<kPair>(at + x_at, &xmap, (s0 + k) * kLinK, m0, bar);
                 ++issued;
                 if (++stage == P.stages) { stage = 0; phase ^= 1u; }
             }
@@ -257,7 +281,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         int stage = 0, n = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
+        for (int u = first; u < units && ok; u += step) {
+            const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
             for (int k0 = 0; k0 < slices && ok; k0 += kLinChunk, ++n) {
                 const int acc = n & 1;
                 if (!lin_wait(sh, &sh.acc_empty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, P.timeout_ns)) {
@@ -292,7 +317,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         const uint32_t d0 = tmem + ((uint32_t)quad << 21) + (uint32_t)c0;
         int n = 0;
         bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
+        for (int u = first; u < units && ok; u += step) {
+            const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
             const int v = t / P.m_tiles * kTileRows + rank * kLinRows + quad * 32 + lane, m0 = t % P.m_tiles * P.cols + c0;
             const int count = min(half, P.M - m0);  // (none for a group whose columns lie behind the batch)
             const bool in = v < P.V;
@@ -327,6 +353,38 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 if (lane == 0) {
                     if constexpr (kPair) arrive_first(&sh.acc_empty[acc]);
                     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.acc_empty[acc])) : "memory");
+                }
+            }
+            if (P.splits > 1) {
+                const int mine = kPair ? 2 * t + rank : t, row = quad * 32 + lane;
+                float* tile = P.partial + (int64_t)mine * P.splits * P.cols * kLinRows + (int64_t)c0 * kLinRows + row;
+                float* to = tile + (int64_t)(u - t * P.splits) * P.cols * kLinRows;
+#pragma unroll
+                for (int c = 0; c < kCols; ++c)
+                    if (ok && c < half) __stcg(to + c * kLinRows, y[c]);
+                // (a warp whose wait ran out takes the others along: none is left waiting at a barrier)
+                if (epilogue_any(!ok, 128 * groups)) ok = false;
+                if (!ok) break;
+                if (tid == 128) {
+                    __threadfence();
+                    const bool last = atomicAdd(&P.tickets[mine], 1u) == (uint32_t)P.splits - 1u;
+                    if (last) {
+                        P.tickets[mine] = 0;
+                        __threadfence();
+                    }
+                    sh.last = last;
+                }
+                asm volatile("bar.sync 1, %0;" ::"r"(128 * groups) : "memory");
+                const bool last = sh.last;
+                asm volatile("bar.sync 1, %0;" ::"r"(128 * groups) : "memory");  // (read by all before the next unit's is written)
+                if (!last) continue;
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) y[c] = 0.0f;
+                for (int s = 0; s < P.splits; ++s) {
+                    const float* from = tile + (int64_t)s * P.cols * kLinRows;
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c)
+                        if (c < half) y[c] += __ldcg(from + c * kLinRows);
                 }
             }
             if (!ok) break;

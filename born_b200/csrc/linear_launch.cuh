@@ -16,9 +16,14 @@ struct LinearArgs {
     const void* residual;
     void* out;
     int64_t x_stride, weight_stride, residual_stride, out_stride;  // elements
+    // scratch for tiles whose K several CTAs share: their sums, and tickets that are 0 between launches
+    float* partial;
+    uint32_t* tickets;
     int* dev_error;
     unsigned long long timeout_ns;
 };
+int64_t linear_scratch_bytes(int num_sms);
+int linear_tickets(int num_sms);
 cudaError_t linear_attrs();
 // dtype: of out and residual
 cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStream_t st);

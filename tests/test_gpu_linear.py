@@ -31,7 +31,8 @@ def whole(shape, seed, lo=-2, hi=3):
 
 @pytest.mark.parametrize("M,K,V", [(1, 8, 1), (1, 16, 7), (2, 56, 127), (3, 64, 128), (15, 72, 129), (16, 128, 1000), (17, 1000, 515),
                                    (64, 512, 18944), (65, 136, 18945), (255, 264, 900), (256, 2048, 640), (257, 64, 300), (300, 192, 19100),
-                                   (512, 320, 400), (700, 64, 257), (1, 8192, 300), (40, 4096, 40000)])
+                                   (512, 320, 400), (700, 64, 257), (1, 8192, 300), (40, 4096, 40000),
+                                   (1, 8192, 1024), (16, 4104, 128), (33, 8000, 130), (128, 2048, 2000), (300, 3200, 1500), (512, 4096, 4096)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_whole_numbers_are_exact(s, M, K, V, dtype):
     import torch
@@ -135,6 +136,16 @@ def test_offsets_past_32_bits(s):
     assert torch.equal(out[:, -1], x.double().sum(1).float())
     assert torch.equal(out[:, 123456], 2 * x[:, :7].double().sum(1).float())
     assert int((out != 0).sum()) <= 4
+
+
+def test_results_do_not_depend_on_the_run(s):
+    """Parts of K are added in their order, whichever CTA comes last."""
+    import torch
+    for M, K, V in [(1, 8192, 1024), (100, 4096, 900)]:
+        x, w = torch.randn((M, K), device="cuda").to(torch.bfloat16), torch.randn((V, K), device="cuda").to(torch.bfloat16)
+        y = s.linear(x, w)
+        for _ in range(5):
+            assert torch.equal(s.linear(x, w), y)
 
 
 def test_graph_and_stream(s):
