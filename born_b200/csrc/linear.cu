@@ -30,17 +30,19 @@ static bool make_map(CUtensorMap* map, const void* p, int rows, int K, int64_t s
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename O, int kCols, bool kPair>
+template <typename O, int kCols, bool kPair, bool kTwo>
 static cudaError_t raise_limit() {
-    return cudaFuncSetAttribute(linear_kernel<O, kCols, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem);
+    return cudaFuncSetAttribute(linear_kernel<O, kCols, kPair, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem);
 }
 template <typename O>
 static cudaError_t raise_limits() {
-    cudaError_t e;
-    if ((e = raise_limit<O, 16, false>()) != cudaSuccess || (e = raise_limit<O, 32, false>()) != cudaSuccess) return e;
-    if ((e = raise_limit<O, 64, false>()) != cudaSuccess || (e = raise_limit<O, 128, false>()) != cudaSuccess) return e;
-    if ((e = raise_limit<O, 64, true>()) != cudaSuccess) return e;
-    return raise_limit<O, 128, true>();
+    const cudaError_t e[] = {raise_limit<O, 16, false, false>(), raise_limit<O, 32, false, false>(), raise_limit<O, 64, false, false>(),
+                             raise_limit<O, 128, false, false>(), raise_limit<O, 64, true, false>(), raise_limit<O, 128, true, false>(),
+                             raise_limit<O, 16, false, true>(), raise_limit<O, 32, false, true>(), raise_limit<O, 64, false, true>(),
+                             raise_limit<O, 128, true, true>()};
+    for (const cudaError_t x : e)
+        if (x != cudaSuccess) return x;
+    return cudaSuccess;
 }
 int64_t linear_scratch_bytes(int num_sms) { return (int64_t)num_sms * kLinSplitCols * kLinRows * 4; }
 int linear_tickets(int num_sms) { return num_sms; }
@@ -49,7 +51,7 @@ cudaError_t linear_attrs() {
     return e != cudaSuccess ? e : raise_limits<__nv_bfloat16>();
 }
 
-template <typename O, int kCols, bool kPair>
+template <typename O, int kCols, bool kPair, bool kTwo>
 static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, unsigned grid, cudaStream_t st) {
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -65,15 +67,20 @@ static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& x, const Line
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = kPair ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair>, w, x, P);
+    return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair, kTwo>, w, x, P);
 }
 template <typename O>
-static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, bool pair, unsigned grid, cudaStream_t st) {
+static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, bool pair, bool two, unsigned grid, cudaStream_t st) {
+    if (two) {
+        if (pair) return launch<O, 128, true, true>(w, x, P, grid, st);
+        if (P.cols <= 16) return launch<O, 16, false, true>(w, x, P, grid, st);
+        return P.cols <= 32 ? launch<O, 32, false, true>(w, x, P, grid, st) : launch<O, 64, false, true>(w, x, P, grid, st);
+    }
     const int cols = P.cols > 16 ? P.cols / 2 : 16;
-    if (pair) return cols <= 64 ? launch<O, 64, true>(w, x, P, grid, st) : launch<O, 128, true>(w, x, P, grid, st);
-    if (cols <= 16) return launch<O, 16, false>(w, x, P, grid, st);
-    if (cols <= 32) return launch<O, 32, false>(w, x, P, grid, st);
-    return cols <= 64 ? launch<O, 64, false>(w, x, P, grid, st) : launch<O, 128, false>(w, x, P, grid, st);
+    if (pair) return cols <= 64 ? launch<O, 64, true, false>(w, x, P, grid, st) : launch<O, 128, true, false>(w, x, P, grid, st);
+    if (cols <= 16) return launch<O, 16, false, false>(w, x, P, grid, st);
+    if (cols <= 32) return launch<O, 32, false, false>(w, x, P, grid, st);
+    return cols <= 64 ? launch<O, 64, false, false>(w, x, P, grid, st) : launch<O, 128, false, false>(w, x, P, grid, st);
 }
 
 cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStream_t st) {
@@ -81,42 +88,55 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStrea
     memset(&P, 0, sizeof P);
     P.M = A.M; P.K = A.K; P.V = A.V;
     P.v_tiles = (A.V + kLinRows - 1) / kLinRows;
-    // as few column tiles as hold the rows, of equal widths; 128 columns at most where the tiles are few
-    const int most = (int64_t)P.v_tiles * ((A.M + kLinMaxCols - 1) / kLinMaxCols) * 2 <= num_sms ? kLinSplitCols : kLinMaxCols;
+    // As few column tiles as hold the rows, of equal widths; narrower ones where the tiles are few (rows x hidden x
+    // features with 256, 128, 64 columns: 128 x 4096 x 4096 27.4, 27.3, 20.2 us; 256 x 8192 x 2000 53, 32, 31;
+    // 512 x 4096 x 4096 31, 29, 37, whose tiles of 64 columns are more than the SMs).
+    int most = kLinMaxCols;
+    if ((int64_t)P.v_tiles * ((A.M + most - 1) / most) * 2 <= num_sms) most = (int64_t)P.v_tiles * ((A.M + 63) / 64) <= num_sms ? 64 : kLinSplitCols;
     P.m_tiles = (A.M + most - 1) / most;
     const int unit = A.M <= 16 ? 16 : 32;  // (a multiple of 16 for either half of the epilogue)
     P.cols = ((A.M + P.m_tiles - 1) / P.m_tiles + unit - 1) / unit * unit;
     P.m_tiles = (A.M + P.cols - 1) / P.cols;
     // A pair from 65 columns on: below that the batch's slices are a third of the bytes at most
     const bool pair = P.cols > 64 && A.V > kLinRows;
-    if (pair) P.v_tiles = (A.V + 2 * kLinRows - 1) / (2 * kLinRows);
+    const int unit_rows = pair ? 2 * kLinRows : kLinRows, room = pair ? num_sms / 2 : num_sms;
+    const int x_rows = pair ? P.cols / 2 : P.cols;  // of the batch in a CTA
+    // Two tiles a CTA (up to 128 columns: tensor memory holds two accumulators of both) where that gives the
+    // busiest SM fewer rows to read, those of the batch included.  Hidden 4096, 128256 features, one tile -> two:
+    // 1 row 161 -> 173 us, 32 rows 184 -> 190, 64 rows 211 -> 194; 2048 x 32000 for 1 row 28.7 -> 24.9.
+    const auto busiest = [&](int rows) {
+        const int64_t units = (int64_t)((A.V + (int64_t)rows * (pair ? 2 : 1) - 1) / (rows * (pair ? 2 : 1))) * P.m_tiles;
+        return (units + room - 1) / room * (rows + x_rows);
+    };
+    const bool two = P.cols <= (pair ? 128 : 64) && busiest(2 * kLinRows) < busiest(kLinRows);
+    P.v_tiles = two ? (A.V + 2 * unit_rows - 1) / (2 * unit_rows) : (A.V + unit_rows - 1) / unit_rows;
     // K is shared out while CTAs are left, in parts of four slices at least; adding up the parts costs the one that
     // does it their bytes, so wide tiles get few
-    const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles, room = pair ? num_sms / 2 : num_sms;
+    const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles;
     const int slices = (A.K + kLinK - 1) / kLinK;
     int64_t splits = room / tiles;
     if (splits > slices / 4) splits = slices / 4;
     if (splits > 1024 / P.cols) splits = 1024 / P.cols;
-    if (splits < 1 || P.cols > kLinSplitCols) splits = 1;
+    if (splits < 1 || two || P.cols > kLinSplitCols) splits = 1;
     P.part = (int)((slices + splits - 1) / splits);
     P.splits = (slices + P.part - 1) / P.part;
     P.partial = A.partial; P.tickets = A.tickets;
-    const int x_rows = pair ? P.cols / 2 : P.cols;  // of the batch in a CTA
-    P.stage_bytes = (kLinRows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
+    const int w_rows = two ? 2 * kLinRows : kLinRows;
+    P.stage_bytes = (w_rows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
     P.stages = (kLinSmem - 1024) / P.stage_bytes;
     if (P.stages > kLinMaxStages) P.stages = kLinMaxStages;
     P.tmem_cols = 32;
-    while (P.tmem_cols < 2 * P.cols) P.tmem_cols *= 2;
+    while (P.tmem_cols < (two ? 4 : 2) * P.cols) P.tmem_cols *= 2;
     P.activation = A.activation; P.scale = A.scale; P.inv_scale = 1.0f / A.scale;
     P.bias = A.bias; P.residual = A.residual; P.out = A.out;
     P.residual_stride = A.residual_stride; P.out_stride = A.out_stride;
     P.dev_error = A.dev_error; P.timeout_ns = A.timeout_ns;
     CUtensorMap w, x;
-    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
+    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, w_rows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
     const int64_t units = tiles * P.splits;
-    const unsigned grid = (unsigned)(units < room ? units : room) * (pair ? 2u : 1u);
-    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, x, P, pair, grid, st);
-    return launch_as<__nv_bfloat16>(w, x, P, pair, grid, st);
+    const unsigned grid = (unsigned)(units < room ? units : (int64_t)room) * (pair ? 2u : 1u);
+    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, x, P, pair, two, grid, st);
+    return launch_as<__nv_bfloat16>(w, x, P, pair, two, grid, st);
 }
 
 }  // namespace born

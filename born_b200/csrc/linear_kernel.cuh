@@ -12,6 +12,10 @@
 // for every 128 rows of weights, and 256 columns of it twice the weights' bytes: out of L2, 256 rows of hidden
 // 4096 over 128256 features took 330 us with that.
 //
+// Up to 128 columns a CTA takes two such tiles at a time (kTwo), 256 v for one slice of the batch: L2 hands out some
+// 8.5 TB/s in all, and the batch's slices count as much as the weights there.  64 rows of hidden 4096, 128256
+// features: 209 us without.
+//
 // The tensor core cuts partial sums off rather than rounding them, once per 16 products, which adds up: 4.3e-6 of
 // the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded.
 //
@@ -199,8 +203,8 @@ __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // kCols: columns of the tile that a thread of the epilogue holds at most (the two groups of four warps take half
-// of the tile's columns each, or the first one all 16).
-template <typename O, int kCols, bool kPair>
+// of the tile's columns each, or the first one all 16; in kTwo a tile each).
+template <typename O, int kCols, bool kPair, bool kTwo>
 __global__ void __launch_bounds__(kLinThreads, 1)
 linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ LinearParams P) {
     extern __shared__ uint8_t raw[];
@@ -211,8 +215,9 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     const int first = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int units = P.v_tiles * P.m_tiles * P.splits;      // tiles, times the parts of K
     const int all_slices = (P.K + kLinK - 1) / kLinK;
-    const int groups = P.cols > 16 ? 2 : 1;                  // of warps that take part in the epilogue
-    constexpr int kTileRows = kPair ? 2 * kLinRows : kLinRows;
+    const int groups = kTwo || P.cols > 16 ? 2 : 1;          // of warps that take part in the epilogue
+    constexpr int kMine = kTwo ? 2 * kLinRows : kLinRows;    // v of this CTA
+    constexpr int kTileRows = kPair ? 2 * kMine : kMine;     // v of a unit
     if (tid == 0) {
         for (int i = 0; i < P.stages; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -240,7 +245,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     if constexpr (kPair) cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sh.tmem;
-    const uint32_t x_at = kLinRows * kLinK * 2;  // the batch's slice behind the weights' one
+    const uint32_t x_at = kMine * kLinK * 2;  // the batch's slice behind the weights' one
+    const int acc_cols = kTwo ? 2 * P.cols : P.cols;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -252,7 +258,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         bool ok = true;
         for (int u = first; u < units && ok; u += step) {
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
-            const int v0 = t / P.m_tiles * kTileRows + rank * kLinRows;
+            const int v0 = t / P.m_tiles * kTileRows + rank * kMine;
             const int m0 = t % P.m_tiles * P.cols + (kPair ? rank * (P.cols / 2) : 0);
             for (int k = 0; k < slices; ++k) {
                 if (!lin_wait(sh, &sh.empty[stage], phase ^ 1u, P.timeout_ns)) {
@@ -277,7 +283,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
         // ---- products: D fp32, A and B bf16, both K-major
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(P.cols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(P.cols >> 3) << 17) | ((uint32_t)((kPair ? 2 * kLinRows : kLinRows) >> 4) << 24);
         int stage = 0, n = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -290,7 +296,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + (uint32_t)(acc * P.cols);
+                const uint32_t d = tmem + (uint32_t)(acc * acc_cols);
                 const int k1 = min(slices, k0 + kLinChunk);
                 for (int k = k0; k < k1; ++k) {
                     if (!lin_wait(sh, &sh.full[stage], phase, P.timeout_ns)) {
@@ -302,6 +308,11 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
 #pragma unroll
                     for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
+                    if constexpr (kTwo) {
+                        const uint64_t a2 = smem_desc(at + kLinRows * kLinK * 2);
+#pragma unroll
+                        for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
+                    }
                     mma_commit<kPair>(&sh.empty[stage]);
                     if (++stage == P.stages) { stage = 0; phase ^= 1u; }
                 }
@@ -313,13 +324,15 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         lin_settle(smem_u32(&sh.drained), 0, P.timeout_ns);
     } else if (warp >= 4 && (warp - 4) >> 2 < groups) {
         // ---- epilogue
-        const int half = P.cols / groups, c0 = ((warp - 4) >> 2) * half, quad = warp & 3;
-        const uint32_t d0 = tmem + ((uint32_t)quad << 21) + (uint32_t)c0;
+        const int group = (warp - 4) >> 2, quad = warp & 3;
+        const int half = kTwo ? P.cols : P.cols / groups, c0 = kTwo ? 0 : group * half;  // its columns
+        const int r0 = (kTwo ? group * kLinRows : 0) + quad * 32 + lane;                 // its v
+        const uint32_t d0 = tmem + ((uint32_t)quad << 21) + (uint32_t)(kTwo ? group * P.cols : c0);
         int n = 0;
         bool ok = true;
         for (int u = first; u < units && ok; u += step) {
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
-            const int v = t / P.m_tiles * kTileRows + rank * kLinRows + quad * 32 + lane, m0 = t % P.m_tiles * P.cols + c0;
+            const int v = t / P.m_tiles * kTileRows + rank * kMine + r0, m0 = t % P.m_tiles * P.cols + c0;
             const int count = min(half, P.M - m0);  // (none for a group whose columns lie behind the batch)
             const bool in = v < P.V;
             const float bias = P.bias && in ? P.bias[v] : 0.0f;
@@ -333,7 +346,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 // (every lane observes the phase itself before it reads what the products wrote)
                 ring_try(smem_u32(&sh.acc_full[acc]), (uint32_t)(n >> 1) & 1u);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = d0 + (uint32_t)(acc * P.cols);
+                const uint32_t d = d0 + (uint32_t)(acc * acc_cols);
 #pragma unroll
                 for (int c = 0; c < kCols; c += 16) {
                     if (c >= half) break;
@@ -355,8 +368,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.acc_empty[acc])) : "memory");
                 }
             }
-            if (P.splits > 1) {
-                const int mine = kPair ? 2 * t + rank : t, row = quad * 32 + lane;
+            if (!kTwo && P.splits > 1) {
+                const int mine = kPair ? 2 * t + rank : t, row = r0;
                 float* tile = P.partial + (int64_t)mine * P.splits * P.cols * kLinRows + (int64_t)c0 * kLinRows + row;
                 float* to = tile + (int64_t)(u - t * P.splits) * P.cols * kLinRows;
 #pragma unroll
