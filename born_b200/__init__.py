@@ -17,3 +17,4 @@ from .sampler import (  # noqa: F401
     load_library,
     version,
 )
+from .beam import BeamSearch, Head  # noqa: F401,E402

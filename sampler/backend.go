@@ -30,6 +30,12 @@ type binding interface {
 	maskBegin(handle uintptr, batch, wordsPerRow int32, host *uintptr) int32
 	maskCommit(handle uintptr, device *uintptr) int32
 	maskWait(handle uintptr, stream uintptr) int32
+	beamStep(handle uintptr, a *BeamArgs, stream uintptr) int32
+	beamNext(handle uintptr, a *BeamArgs, stream uintptr) int32
+	beamPoolReset(handle uintptr, a *BeamArgs, stream uintptr) int32
+	beamReorder(handle uintptr, a *ReorderArgs, stream uintptr) int32
+	beamSequences(handle uintptr, a *SequencesArgs, stream uintptr) int32
+	linear(handle uintptr, a *LinearArgs, stream uintptr) int32
 	lastError(handle uintptr) string
 	version() string
 }

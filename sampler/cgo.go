@@ -79,5 +79,23 @@ func (cgoBinding) maskCommit(h uintptr, device *uintptr) int32 {
 	return int32(C.born_mask_commit(h2p(h), (**C.uint32_t)(unsafe.Pointer(device))))
 }
 func (cgoBinding) maskWait(h uintptr, st uintptr) int32 { return int32(C.born_mask_wait(h2p(h), h2p(st))) }
+func (cgoBinding) beamStep(h uintptr, a *BeamArgs, st uintptr) int32 {
+	return int32(C.born_beam_step(h2p(h), (*C.born_beam_args)(unsafe.Pointer(a)), h2p(st)))
+}
+func (cgoBinding) beamNext(h uintptr, a *BeamArgs, st uintptr) int32 {
+	return int32(C.born_beam_next(h2p(h), (*C.born_beam_args)(unsafe.Pointer(a)), h2p(st)))
+}
+func (cgoBinding) beamPoolReset(h uintptr, a *BeamArgs, st uintptr) int32 {
+	return int32(C.born_beam_pool_reset(h2p(h), (*C.born_beam_args)(unsafe.Pointer(a)), h2p(st)))
+}
+func (cgoBinding) beamReorder(h uintptr, a *ReorderArgs, st uintptr) int32 {
+	return int32(C.born_beam_reorder(h2p(h), (*C.born_reorder_args)(unsafe.Pointer(a)), h2p(st)))
+}
+func (cgoBinding) beamSequences(h uintptr, a *SequencesArgs, st uintptr) int32 {
+	return int32(C.born_beam_sequences(h2p(h), (*C.born_sequences_args)(unsafe.Pointer(a)), h2p(st)))
+}
+func (cgoBinding) linear(h uintptr, a *LinearArgs, st uintptr) int32 {
+	return int32(C.born_linear(h2p(h), (*C.born_linear_args)(unsafe.Pointer(a)), h2p(st)))
+}
 func (cgoBinding) lastError(h uintptr) string { return C.GoString(C.born_last_error(h2p(h))) }
 func (cgoBinding) version() string            { return C.GoString(C.born_version()) }

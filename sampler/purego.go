@@ -38,6 +38,12 @@ type puregoBinding struct {
 	fMaskBegin     func(h uintptr, batch, words int32, host *uintptr) int32
 	fMaskCommit    func(h uintptr, device *uintptr) int32
 	fMaskWait      func(h uintptr, stream uintptr) int32
+	fBeamStep      func(h uintptr, a *BeamArgs, stream uintptr) int32
+	fBeamNext      func(h uintptr, a *BeamArgs, stream uintptr) int32
+	fBeamPoolReset func(h uintptr, a *BeamArgs, stream uintptr) int32
+	fBeamReorder   func(h uintptr, a *ReorderArgs, stream uintptr) int32
+	fBeamSequences func(h uintptr, a *SequencesArgs, stream uintptr) int32
+	fLinear        func(h uintptr, a *LinearArgs, stream uintptr) int32
 	fLastError     func(h uintptr) *byte
 	fVersion       func() *byte
 }
@@ -82,6 +88,12 @@ func load() (binding, error) {
 		purego.RegisterLibFunc(&b.fMaskBegin, lib, "born_mask_begin")
 		purego.RegisterLibFunc(&b.fMaskCommit, lib, "born_mask_commit")
 		purego.RegisterLibFunc(&b.fMaskWait, lib, "born_mask_wait")
+		purego.RegisterLibFunc(&b.fBeamStep, lib, "born_beam_step")
+		purego.RegisterLibFunc(&b.fBeamNext, lib, "born_beam_next")
+		purego.RegisterLibFunc(&b.fBeamPoolReset, lib, "born_beam_pool_reset")
+		purego.RegisterLibFunc(&b.fBeamReorder, lib, "born_beam_reorder")
+		purego.RegisterLibFunc(&b.fBeamSequences, lib, "born_beam_sequences")
+		purego.RegisterLibFunc(&b.fLinear, lib, "born_linear")
 		purego.RegisterLibFunc(&b.fLastError, lib, "born_last_error")
 		purego.RegisterLibFunc(&b.fVersion, lib, "born_version")
 		loaded = b
@@ -141,3 +153,9 @@ func (b *puregoBinding) maskBegin(h uintptr, batch, words int32, host *uintptr) 
 }
 func (b *puregoBinding) maskCommit(h uintptr, device *uintptr) int32 { return b.fMaskCommit(h, device) }
 func (b *puregoBinding) maskWait(h uintptr, st uintptr) int32        { return b.fMaskWait(h, st) }
+func (b *puregoBinding) beamStep(h uintptr, a *BeamArgs, st uintptr) int32 { return b.fBeamStep(h, a, st) }
+func (b *puregoBinding) beamNext(h uintptr, a *BeamArgs, st uintptr) int32 { return b.fBeamNext(h, a, st) }
+func (b *puregoBinding) beamPoolReset(h uintptr, a *BeamArgs, st uintptr) int32 { return b.fBeamPoolReset(h, a, st) }
+func (b *puregoBinding) beamReorder(h uintptr, a *ReorderArgs, st uintptr) int32 { return b.fBeamReorder(h, a, st) }
+func (b *puregoBinding) beamSequences(h uintptr, a *SequencesArgs, st uintptr) int32 { return b.fBeamSequences(h, a, st) }
+func (b *puregoBinding) linear(h uintptr, a *LinearArgs, st uintptr) int32 { return b.fLinear(h, a, st) }

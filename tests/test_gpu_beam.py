@@ -618,3 +618,100 @@ def test_refusals(s):
     bad(*inv, s.beam_sequences, t.long(), t, e, e, e, K)
     e17 = torch.zeros((2, 17), **i32)
     bad(*uns, s.beam_sequences, t, t, e17, e17, e17, K)
+
+
+# ---- the search path --------------------------------------------------------------------------
+@pytest.mark.parametrize("history", [0, 16])
+@pytest.mark.parametrize("side", [False, True])
+def test_search_path(s, history, side):
+    """BeamSearch over a head: hidden states are rows of a table picked by the last token, so that the definition can
+    follow; whole numbers in the table and the head make the logits exact."""
+    import torch
+    from born_b200 import BeamConfig, BeamSearch, Head
+    N, K, V, D, steps, stops = 3, 4, 300, 64, 12, (5, 6)
+    rng = np.random.default_rng(31)
+    hid = rng.integers(-3, 4, (V, D)).astype(np.float32)
+    w = rng.integers(-3, 4, (V, D)).astype(np.float32)
+    bias = (rng.standard_normal(V) * 8 - 60).astype(np.float32)
+    bias[list(stops)] += 30
+    T = 7.0
+    pen = dict(repetition=1.3, presence=2.0) if history else {}
+    cfg = BeamConfig(temperature=T, stop_tokens=stops, length_penalty=0.8, keep_slots=True,
+                     repetition_penalty=pen.get("repetition", 0.0), presence_penalty=pen.get("presence", 0.0))
+    head = Head(dev(w).to(torch.bfloat16), dev(bias))
+    table = dev(hid).to(torch.bfloat16)
+    st = torch.cuda.Stream() if side else torch.cuda.default_stream()
+    raw = st.cuda_stream if side else None
+    prompts = rng.integers(0, V, (N, 5)).astype(np.int32)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        search = BeamSearch(s, N, K, steps, V, cfg, head=head, history=history)
+        cache = torch.zeros((N * K, 2, steps, 3), device="cuda")
+        flat = torch.zeros((N * K, 7), device="cuda", dtype=torch.int32)
+        search.begin(dev(prompts) if history else None, stream=raw)
+        last = torch.arange(N, device="cuda").repeat_interleave(K) + 11
+        for t in range(steps):
+            cache[:, :, t] = last.float()[:, None, None]
+            used = torch.full((N,), t + 1, dtype=torch.int32, device="cuda")
+            search.step(table[last], states=[cache], lens=used, position_dim=2, stream=raw)
+            s.beam_reorder([flat], search.parent_table[t], K, stream=raw)
+            last = search.tokens.clamp(min=0).long()
+        found = search.result(stream=raw)
+    torch.cuda.synchronize()
+    got = {k: v.cpu().numpy() for k, v in found.items()}
+    cache = cache.cpu().numpy()
+    for n in range(N):
+        beams = [([], 0.0)] + [([], -np.inf)] * (K - 1)
+        ref, kept = R.Pool(K), {}
+        fed = [[] for _ in range(K)]
+        for t in range(steps):
+            if ref.done:
+                break
+            rows = []
+            for b in range(K):
+                at = beams[b][0][-1] if beams[b][0] else n + 11
+                row = (hid[at] @ w.T + bias).astype(np.float32)
+                if history:
+                    row = R.penalised(row, (list(prompts[n]) + beams[b][0])[-history:], **pen)
+                rows.append(row)
+            out = R.step(rows, [np.float32(b[1]) for b in beams], stops, T, True)
+            fed = [fed[p] + [beams[p][0][-1] if beams[p][0] else n + 11] for p in out["parent"]]
+            for p, k in zip(out["end_parent"], out["end_token"]):
+                if k >= 0:
+                    kept[(t, p, k)] = beams[p][0] + [k]
+            ref.add(out, t, 0.8, False)
+            beams = [((beams[p][0] + [k]) if k >= 0 else beams[p][0], v) for p, k, v in zip(out["parent"], out["token"], out["score"])]
+        want = [(float(v), kept[(t, p, k)]) for v, t, p, k in ref.items]
+        if not ref.done:
+            want += [(v / steps ** np.float64(np.float32(0.8)), q) for q, v in beams if np.isfinite(v)]
+            for b in range(K):  # the caches followed the beams that were fed
+                assert cache[n * K + b, 0, :, 0].tolist() == fed[b], (n, b)
+        want.sort(key=lambda x: -x[0])
+        for i, (v, q) in enumerate(want[:K]):
+            assert got["lens"][n, i] == len(q) and got["tokens"][n, i, :len(q)].tolist() == q, (n, i)
+            # every step rounds the running score once, the normalised one is rounded twice
+            assert abs(got["scores"][n, i] - v) <= steps * score_error(V) + (steps + 2) * abs(v) * len(q) * 2.0 ** -24
+        for i in range(len(want), K):
+            assert got["lens"][n, i] == 0 and got["scores"][n, i] == -np.inf
+
+
+def test_search_refusals(s):
+    import torch
+    from born_b200 import BeamConfig, BeamSearch, Head, InvalidArgument
+    with pytest.raises(InvalidArgument):
+        BeamSearch(s, 2, 4, 5, 100, BeamConfig(presence_penalty=1.0))
+    with pytest.raises(InvalidArgument):
+        BeamSearch(s, 0, 4, 5, 100)
+    with pytest.raises(InvalidArgument):
+        BeamSearch(s, 2, 4, 5, 100, head=Head(torch.zeros((99, 64), dtype=torch.bfloat16, device="cuda")))
+    b = BeamSearch(s, 2, 4, 1, 100)
+    z = torch.zeros((8, 100), device="cuda")
+    for f in (lambda: b.step(z), lambda: b.tokens, b.result):
+        with pytest.raises(InvalidArgument):
+            f()
+    b.begin()
+    with pytest.raises(InvalidArgument):
+        b.step(z[:4])
+    b.step(z)
+    with pytest.raises(InvalidArgument):
+        b.step(z)
