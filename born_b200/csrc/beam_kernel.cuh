@@ -79,6 +79,12 @@ struct BeamShared {
     int last[kBeamSegs];            // the group whose last ticket this was, -1 = none
 };
 
+__device__ __forceinline__ uint32_t smem_atom_and(uint32_t at, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.shared.and.b32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
+    return old;
+}
+
 template <typename T> __device__ __forceinline__ float logit_at(const T* p);
 template <> __device__ __forceinline__ float logit_at<float>(const float* p) { return __ldg(p); }
 template <> __device__ __forceinline__ float logit_at<uint16_t>(const uint16_t* p) { return bf16_bits_to_f32(__ldg(p)); }
@@ -132,16 +138,21 @@ struct BeamSum {
     }
     // two values of z - z0
     __device__ __forceinline__ float2 two(float2 z) const {
-        const float magic = (float)(12582912 - m);  // 1.5 * 2^23: a whole number n comes out as n - m in the low bits
+        const float magic = (float)(12582912 + m);  // 1.5 * 2^23: magic - n has m - n in its low bits
         z.x = fmaxf(z.x, least);
         z.y = fmaxf(z.y, least);
-        const float2 r = __ffma2_rn(z, make_float2(c, c), make_float2(magic, magic));
-        const float2 n = __fadd2_rn(r, make_float2(-magic, -magic));
-        float2 f = __ffma2_rn(z, make_float2(c, c), make_float2(-n.x, -n.y));
+        // (-c and -n rather than n: a packed operation has no sign to flip its operands with)
+        const float2 r = __ffma2_rn(z, make_float2(-c, -c), make_float2(magic, magic));
+        const float2 minus_n = __fadd2_rn(r, make_float2(-magic, -magic));
+        float2 f = __ffma2_rn(z, make_float2(c, c), minus_n);
         f = __ffma2_rn(z, make_float2(c_lo, c_lo), f);
-        // (what is above those bits shifts out)
-        return make_float2(__uint_as_float(__float_as_uint(ex2_approx(f.x)) + (__float_as_uint(r.x) << 23)),
-                           __uint_as_float(__float_as_uint(ex2_approx(f.y)) + (__float_as_uint(r.y) << 23)));
+        return make_float2(scaled(ex2_approx(f.x), r.x), scaled(ex2_approx(f.y), r.y));
+    }
+    // n - m into the exponent: minus r's low bits (what is above them shifts out), in one multiply-add
+    static __device__ __forceinline__ float scaled(float e, float r) {
+        uint32_t o;
+        asm("mad.lo.u32 %0, %1, 0xff800000, %2;" : "=r"(o) : "r"(__float_as_uint(r)), "r"(__float_as_uint(e)));
+        return __uint_as_float(o);
     }
     template <int N>
     __device__ __forceinline__ void add(float (&v)[N], float mx) {
@@ -536,7 +547,7 @@ __device__ __forceinline__ void extend_row(const BeamArgs& A, int b, double boun
 
 // The group's last CTA: merges the records, ranks, arranges, writes.
 template <typename T>
-__device__ __noinline__ void finish_group(const BeamArgs& A, int n, BeamShared& sh, uint32_t* bits) {
+__device__ __forceinline__ void finish_group(const BeamArgs& A, int n, BeamShared& sh, uint32_t* bits) {
     const int K = A.K;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool done = A.done && A.done[n];
@@ -638,7 +649,7 @@ __device__ __forceinline__ uint32_t in_load_order(uint32_t w) {
 // The K best tokens of a segment by K rounds over all its values: where the candidates overflow, as when a
 // few threads hold nearly all the large values.  key_of(i), i < count, enumerates the calling thread's keys (0: none).
 template <typename F>
-__device__ __noinline__ void slow_list(unsigned long long* scratch, unsigned long long* list, int K, int count, const F& key_of) {
+__device__ __forceinline__ void slow_list(unsigned long long* scratch, unsigned long long* list, int K, int count, const F& key_of) {
     unsigned long long below = ~0ull;
     for (int k = 0; k < K; ++k) {
         unsigned long long best = 0;
@@ -749,16 +760,21 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
         __syncthreads();
         // ---- their bits and histories, and the stop tokens' logits
         constexpr int kIds = BORN_MAX_HISTORY / kThreads;
-        int32_t id[kBeamSegs][kIds];
         if (hist) {
+            int32_t id[kBeamSegs][kIds];
 #pragma unroll
             for (int g = 0; g < kBeamSegs; ++g) {
                 const int64_t row = g < ns ? sh.sg[g].row : -1;
-                const int len = row < 0 ? 0 : max(0, min(A.history_len ? A.history_len[row] : A.history_stride, A.history_stride));
-                if (tid == 0) sh.sg[g].n_own = len;
 #pragma unroll
-                for (int j = 0; j < kIds; ++j) id[g][j] = tid + j * kThreads < len ? A.history[row * A.history_stride + tid + j * kThreads] : -1;
+                for (int j = 0; j < kIds; ++j)
+                    id[g][j] = row >= 0 && tid + j * kThreads < A.history_stride ? A.history[row * A.history_stride + tid + j * kThreads] : -1;
+                if (tid == 0) sh.sg[g].n_own = row < 0 ? 0 : max(0, min(A.history_len ? A.history_len[row] : A.history_stride, A.history_stride));
             }
+#pragma unroll
+            for (int g = 0; g < kBeamSegs; ++g)
+#pragma unroll
+                for (int j = 0; j < kIds; ++j)
+                    if (tid + j * kThreads < A.hist_cap) own[g * A.hist_cap + tid + j * kThreads] = id[g][j];
         }
         if constexpr (kBits) {
 #pragma unroll 1
@@ -789,24 +805,26 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
             if (hist) {
                 // whoever clears a token's bit owns it; later occurrences are listed, to be counted; masked tokens are
                 // taken for later occurrences of nothing
-#pragma unroll
-                for (int g = 0; g < kBeamSegs; ++g) {
-                    if (g >= ns) continue;
+                const uint32_t bits0_at = smem_u32(bits);
+#pragma unroll 1
+                for (int g = 0; g < ns; ++g) {
                     auto& G = sh.sg[g];
+                    const int o0 = (G.s0 - bits0) * kBlkTok - G.lo, len = G.n_own;
+                    int32_t* ids = own + g * A.hist_cap + tid;
+                    int32_t t[kIds];
+                    uint32_t was[kIds];
 #pragma unroll
                     for (int j = 0; j < kIds; ++j) {
-                        int t = id[g][j];
-                        if (t >= G.lo && t < G.hi) {
-                            const int o = (G.s0 - bits0) * kBlkTok + t - G.lo;
-                            const uint32_t bit = 1u << (o & 31);
-                            if (!(atomicAnd(&bits[o >> 5], ~bit) & bit)) {
-                                dups[g * A.hist_cap + atomicAdd(&G.n_dups, 1)] = t;
-                                t = -1;
-                            }
-                        } else {
-                            t = -1;
-                        }
-                        if (tid + j * kThreads < A.hist_cap) own[g * A.hist_cap + tid + j * kThreads] = t;
+                        t[j] = tid + j * kThreads < len ? ids[j * kThreads] : -1;
+                        const int o = o0 + t[j];
+                        if (t[j] < G.lo || t[j] >= G.hi) t[j] = -1;
+                        else was[j] = smem_atom_and(bits0_at + (uint32_t)(o >> 5) * 4u, ~(1u << (o & 31))) >> (o & 31);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kIds; ++j) {
+                        const bool again = t[j] >= 0 && !(was[j] & 1u);
+                        if (again) dups[g * A.hist_cap + atomicAdd(&G.n_dups, 1)] = t[j];
+                        if (tid + j * kThreads < len && (again || t[j] < 0)) ids[j * kThreads] = -1;
                     }
                 }
                 __syncthreads();
