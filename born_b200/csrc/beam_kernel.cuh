@@ -413,28 +413,20 @@ __device__ __noinline__ void move_history(const BeamArgs& A, const BeamShared& s
 
 // The records of a row, a warp over them: lane i walks down the list of record i.
 struct RowHeads {
-    const BeamRecord* r;
-    unsigned long long h, h1, h2, h3;
-    int at;
-    // everything of a record in one round trip, the list's first four entries too
-    __device__ __forceinline__ void load_list(const BeamRecord* rec, bool has, int K) {
-        r = rec;
-        ulonglong2 a = make_ulonglong2(0, 0), b = a;
-        if (has) {
-            a = __ldcg(reinterpret_cast<const ulonglong2*>(rec->list));
-            if (K > 2) b = __ldcg(reinterpret_cast<const ulonglong2*>(rec->list) + 1);
-        }
+    unsigned long long h, next;  // the list's entry, and the one behind it
+    int rec, at;                 // the lane's record; entry behind those
+    // (the list's first two entries, with everything else of a record in one round trip)
+    __device__ __forceinline__ void load_list(const BeamArgs& A, int i, bool has) {
+        rec = i;
+        ulonglong2 a = make_ulonglong2(0, 0);
+        if (has) a = __ldcg(reinterpret_cast<const ulonglong2*>(A.records[i].list));
         h = a.x;
-        h1 = K > 1 ? a.y : 0;
-        h2 = K > 2 ? b.x : 0;
-        h3 = K > 3 ? b.y : 0;
-        at = 4;
+        next = A.K > 1 ? a.y : 0;
+        at = 2;
     }
-    __device__ __forceinline__ void step(int K) {
-        h = h1;
-        h1 = h2;
-        h2 = h3;
-        h3 = h3 && at < K ? __ldcg(&r->list[at]) : 0;
+    __device__ __forceinline__ void step(const BeamArgs& A) {
+        h = next;
+        next = next && at < A.K ? __ldcg(&A.records[rec].list[at]) : 0;
         ++at;
     }
 };
@@ -461,7 +453,7 @@ __device__ __forceinline__ bool merge_row(const BeamArgs& A, int n, int b, bool 
         rm = __ldcg(&r->m);
         rz0 = __ldcg(&r->z0);
     }
-    heads.load_list(r, has, K);
+    heads.load_list(A, first + lane, has);
     if (lane < A.n_stop) {
         const int blk = A.stop_ids[lane] / kBlkTok;
         stop = __ldcg(&A.records[A.record_of((q0 + blk / A.pb) * A.pb + blk % A.pb)].stop_z[lane]);
@@ -489,14 +481,14 @@ __device__ __forceinline__ bool merge_row(const BeamArgs& A, int n, int b, bool 
             if (src == 32) break;
             const unsigned long long best = __shfl_sync(0xffffffffu, heads.h, src);
             if (lane == k) kept = best;
-            if (lane == src) heads.step(K);
+            if (lane == src) heads.step(A);
         }
         for (int base = first + 32; base <= last; base += 32) {
             // the best of the records before are a 33rd list
             const bool more = base + lane <= last;
             r = A.records + base + lane;
             if (more) s += in_units(A, __ldcg(&r->sum), __ldcg(&r->m), __ldcg(&r->z0), m1, z1);
-            heads.load_list(r, more, K);
+            heads.load_list(A, base + lane, more);
             const unsigned long long old = kept;
             int at_old = 0;
             kept = 0;
@@ -506,7 +498,7 @@ __device__ __forceinline__ bool merge_row(const BeamArgs& A, int n, int b, bool 
                 if (best == 0) break;
                 if (lane == k) kept = best;
                 if (prev == best) ++at_old;
-                else if (heads.h == best) heads.step(K);
+                else if (heads.h == best) heads.step(A);
             }
         }
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -538,7 +530,7 @@ __device__ __forceinline__ void extend_row(const BeamArgs& A, int b, double boun
             ends = !(v >= bound);
             if (!ends) {
                 sh.row_list[b][k] = heads.h;
-                heads.step(K);
+                heads.step(A);
             }
         }
         if (__any_sync(0xffffffffu, ends)) break;
@@ -963,12 +955,11 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
         }
         __syncthreads();
 
-        // ---- every warp: the segments' maxima and the keys that at least K + n_stop tokens reach; a share of the
-        // groups that reach them
-#pragma unroll 1
-        for (int g = 0; g < ns; ++g) {
+        // ---- a team of warps per segment: every warp its maximum and the key that at least K + n_stop tokens reach; a
+        // share of the groups that reach it
+        const int team = warp % ns, crew = kThreads / ns, me = warp / ns * 32 + lane;
+        if (const int g = team; sh.sg[g].row >= 0) {
             auto& G = sh.sg[g];
-            if (G.row < 0) continue;
             float bm = -INFINITY;
             if (lane < kBeamWarps) {
                 bm = G.wmax[lane];
@@ -1004,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                 one.m = m1;
                 one.least = __fdividef((float)m1 - 100.0f, one.c);
                 unsigned long long u = 0;
-                for (int i = tid; i < G.n_own; i += kThreads) {
+                for (int i = me; i < G.n_own; i += crew) {
                     const float x = own[g * A.hist_cap + i] >= 0 ? own_z[g * A.hist_cap + i] : -INFINITY;
                     if (!(x > -INFINITY)) continue;
                     u += __float2ull_rn(one.two(make_float2(x - z1, x - z1)).x * 1099511627776.0f);
@@ -1015,7 +1006,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
             }
             const uint32_t least = max((uint32_t)(bound >> 40), 0x80u);  // (0x7f is -inf)
             const int groups = (G.hi - G.lo + 31) / 32, first = (G.s0 - bits0) * 32;
-            for (int i = tid; i < groups; i += kThreads) {
+            for (int i = me; i < groups; i += crew) {
                 if (gkey[first + i] < least) continue;
                 const int at = atomicAdd(&G.n_groups, 1);
                 if (at < kBeamGroups) sh.seg[g].groups[at] = (uint16_t)i;
@@ -1043,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                     if (lane < BORN_MAX_BEAMS) gap->list[lane] = 0;
                 }
             }
-            if (lane == 0 && warp == 0) sh.seg[g].pool[kBeamPool - 1] = bound;
+            if (lane == 0 && warp == g) sh.seg[g].pool[kBeamPool - 1] = bound;
         }
         __syncthreads();
         // rank key of token `tok` of segment g, 0 = none
@@ -1057,14 +1048,12 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
             const float x = logit_at<T>(reinterpret_cast<const T*>(A.logits) + G.row * A.row_stride + tok);
             return x > -INFINITY ? (unsigned long long)make_ck(x, tok) : 0ull;
         };
-#pragma unroll 1
-        for (int g = 0; g < ns; ++g) {
+        if (const int g = team; sh.sg[g].row >= 0) {
             auto& G = sh.sg[g];
-            if (G.row < 0) continue;
             const unsigned long long bound = sh.seg[g].pool[kBeamPool - 1];
-            if (tid == 32 * g && hist) A.records[(int)blockIdx.x + G.q].sum += (double)G.hist_mass * 0x1p-40;
+            if (warp == g && lane == 0 && hist) A.records[(int)blockIdx.x + G.q].sum += (double)G.hist_mass * 0x1p-40;
             const int listed = min(G.n_groups, kBeamGroups);
-            for (int i = warp; i < listed; i += kBeamWarps) {
+            for (int i = me >> 5; i < listed; i += crew >> 5) {
                 const unsigned long long k = key_at(g, G.lo + (int)sh.seg[g].groups[i] * 32 + lane);
                 if (k < bound || is_stop(A, ck_idx(k))) continue;
                 const int at = atomicAdd(&G.n_cand, 1);
@@ -1072,30 +1061,30 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
             }
         }
         __syncthreads();
+        const auto fits = [&](int g) { return sh.sg[g].n_cand <= kBeamCand && sh.sg[g].n_groups <= kBeamGroups; };
+        if (const int g = team; sh.sg[g].row >= 0 && fits(g)) {
+            unsigned long long* list = A.records[(int)blockIdx.x + sh.sg[g].q].list;
+            const int found = sh.sg[g].n_cand;
+            for (int i = me; i < found; i += crew) {
+                const unsigned long long k = sh.seg[g].cand[i];
+                int ahead = 0;
+                for (int j = 0; j < found; ++j) ahead += sh.seg[g].cand[j] > k;
+                if (ahead < K) list[ahead] = k;
+            }
+            if (me >= found && me < K) list[me] = 0;
+        }
 #pragma unroll 1
         for (int g = 0; g < ns; ++g) {
             const auto& G = sh.sg[g];
-            if (G.row < 0) continue;
-            unsigned long long* list = A.records[(int)blockIdx.x + G.q].list;
-            const int found = G.n_cand;
-            if (found <= kBeamCand && G.n_groups <= kBeamGroups) {
-                for (int i = tid; i < found; i += kThreads) {
-                    const unsigned long long k = sh.seg[g].cand[i];
-                    int ahead = 0;
-                    for (int j = 0; j < found; ++j) ahead += sh.seg[g].cand[j] > k;
-                    if (ahead < K) list[ahead] = k;
-                }
-                if (tid >= found && tid < K) list[tid] = 0;
-            } else {
-                const int most = (G.hi - G.lo + kThreads - 1) / kThreads;
-                slow_list(sh.seg[g].pool, list, K, most + (hist ? BORN_MAX_HISTORY / kThreads : 0), [&](int i) {
-                    unsigned long long k = 0;
-                    if (i < most) k = key_at(g, G.lo + i * kThreads + tid);
-                    else if (const int e = (i - most) * kThreads + tid; e < G.n_own && own[g * A.hist_cap + e] >= 0 && own_z[g * A.hist_cap + e] > -INFINITY)
-                        k = make_ck(own_z[g * A.hist_cap + e], own[g * A.hist_cap + e]);
-                    return k && !is_stop(A, ck_idx(k)) ? k : 0ull;
-                });
-            }
+            if (G.row < 0 || fits(g)) continue;
+            const int most = (G.hi - G.lo + kThreads - 1) / kThreads;
+            slow_list(sh.seg[g].pool, A.records[(int)blockIdx.x + G.q].list, K, most + (hist ? BORN_MAX_HISTORY / kThreads : 0), [&](int i) {
+                unsigned long long k = 0;
+                if (i < most) k = key_at(g, G.lo + i * kThreads + tid);
+                else if (const int e = (i - most) * kThreads + tid; e < G.n_own && own[g * A.hist_cap + e] >= 0 && own_z[g * A.hist_cap + e] > -INFINITY)
+                    k = make_ck(own_z[g * A.hist_cap + e], own[g * A.hist_cap + e]);
+                return k && !is_stop(A, ck_idx(k)) ? k : 0ull;
+            });
         }
         __syncthreads();
         // ---- the groups' tickets, which count blocks
