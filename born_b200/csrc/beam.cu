@@ -6,14 +6,16 @@
 
 namespace born {
 
-static void row_pieces(int vocab, int& pieces, int& pb) {
+// The fewest pieces of at most `most` blocks.
+static void row_pieces(int vocab, int most, int& pieces, int& pb) {
     const int nb = (vocab + kBlkTok - 1) / kBlkTok;
-    pieces = (nb + kBeamPiece - 1) / kBeamPiece;
+    pieces = (nb + most - 1) / most;
     pb = (nb + pieces - 1) / pieces;
 }
+constexpr int kBeamLeastPiece = 48;  // blocks that a piece is not cut below for the sake of a longer ring
 int64_t beam_max_records(int max_batch, int max_vocab, int num_sms) {
     int pieces, pb;
-    row_pieces(max_vocab, pieces, pb);
+    row_pieces(max_vocab, kBeamLeastPiece, pieces, pb);
     return 2 * (int64_t)num_sms + (int64_t)max_batch * (pieces + 1);  // (CTAs and pieces; a CTA of its own for every piece)
 }
 
@@ -69,26 +71,33 @@ static cudaError_t beam_launch_as(const BeamArgs& A, bool has_bits, bool aligned
 
 cudaError_t beam_launch(BeamArgs& A, int dtype, bool aligned, int num_sms, cudaStream_t st) {
     const bool has_bits = A.mask || A.history;
-    row_pieces(A.V, A.pieces, A.pb);
-    const int64_t rows = (int64_t)A.N * A.K, pieces = rows * A.pieces, blocks = pieces * A.pb;
-    if (blocks > 0x7fffffff / kBlkTok) return cudaErrorInvalidValue;
-    A.blocks = (int)blocks;
-    // a block per warp at least, a CTA of its own for every piece while the GPU holds them at once
-    int64_t grid = (blocks + kBeamWarps - 1) / kBeamWarps;
-    if (grid < pieces) grid = pieces;
-    if (grid > 2 * num_sms) grid = 2 * num_sms;
-    A.grid = (int)grid;
-    const int range = (int)((blocks + grid - 1) / grid), seg = range < kBeamSegs * A.pb ? range : kBeamSegs * A.pb;  // blocks taken at a time
     const int esz = dtype == BORN_DTYPE_F32 ? 4 : 2;
-    const int bit_bytes = has_bits ? seg * 128 : 0, key_bytes = (seg * 64 + 127) & ~127;
-    A.bit_words = bit_bytes / 4;
     A.slot_bytes = ring_slot_bytes(esz, aligned);
     A.hist_cap = A.history ? (A.history_stride + 31) / 32 * 32 : 0;  // ids, penalised logits and later occurrences of each segment
     const int hist_bytes = kBeamSegs * A.hist_cap * 12;
-    A.slots = (kBeamSmem - bit_bytes - key_bytes - hist_bytes) / (kBeamWarps * A.slot_bytes);
-    const int most = (range + kBeamWarps - 1) / kBeamWarps;
-    if (A.slots > most) A.slots = most;
-    if (A.slots > kBeamMaxSlots) A.slots = kBeamMaxSlots;
+    int bit_bytes = 0, key_bytes = 0;
+    // as few pieces as possible, more where two segments' bits and keys would leave a warp fewer than two ring slots
+    for (int most = kBeamPiece;; most = most * 3 / 4 > kBeamLeastPiece ? most * 3 / 4 : kBeamLeastPiece) {
+        row_pieces(A.V, most, A.pieces, A.pb);
+        const int64_t pieces = (int64_t)A.N * A.K * A.pieces, blocks = pieces * A.pb;
+        if (blocks > 0x7fffffff / kBlkTok) return cudaErrorInvalidValue;
+        A.blocks = (int)blocks;
+        // a block per warp at least, a CTA of its own for every piece while the GPU holds them at once
+        int64_t grid = (blocks + kBeamWarps - 1) / kBeamWarps;
+        if (grid < pieces) grid = pieces;
+        if (grid > 2 * num_sms) grid = 2 * num_sms;
+        A.grid = (int)grid;
+        const int range = (int)((blocks + grid - 1) / grid), seg = range < kBeamSegs * A.pb ? range : kBeamSegs * A.pb;  // blocks taken at a time
+        bit_bytes = has_bits ? seg * 128 : 0;
+        key_bytes = (seg * 64 + 127) & ~127;
+        A.slots = (kBeamSmem - bit_bytes - key_bytes - hist_bytes) / (kBeamWarps * A.slot_bytes);
+        const int need = (range + kBeamWarps - 1) / kBeamWarps;
+        if (A.slots > need) A.slots = need;
+        if (A.slots > kBeamMaxSlots) A.slots = kBeamMaxSlots;
+        if (A.slots >= (need < 2 ? need : 2) || most == kBeamLeastPiece) break;
+    }
+    if (A.slots < 1) return cudaErrorInvalidValue;
+    A.bit_words = bit_bytes / 4;
     A.bits_at = kBeamWarps * A.slots * A.slot_bytes;
     A.gkeys_at = A.bits_at + bit_bytes;
     A.slack = beam_slack();

@@ -48,7 +48,6 @@ struct BeamShared {
             unsigned long long row_list[BORN_MAX_BEAMS][BORN_MAX_BEAMS];  // the rows' best tokens, 0-terminated
             double value[BORN_MAX_BEAMS * (BORN_MAX_BEAMS + BORN_MAX_STOPS)];  // of the candidates
             uint32_t flat[BORN_MAX_BEAMS * (BORN_MAX_BEAMS + BORN_MAX_STOPS)]; // beam << 24 | token, kStopBit: a stop token
-            int32_t hist[BORN_MAX_HISTORY];
         };
     };
     struct {
@@ -201,7 +200,7 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
 // log sum exp((z - m)/T) of a row in 64 bits, by the whole CTA, in an order that depends on the token
 // indices alone (equal rows give equal bits).  Rare, and slow: tens of microseconds for a row of 128256 tokens.
 template <typename T>
-__device__ __noinline__ double row_normaliser(const BeamArgs& A, int64_t row, float m, BeamShared& sh, uint32_t* bits) {
+__device__ __noinline__ double row_normaliser(const BeamArgs& A, int64_t row, float m, BeamShared& sh, uint32_t* bits, int32_t* hist) {
     const T* z = reinterpret_cast<const T*>(A.logits) + row * A.row_stride;
     const double invT = A.inv_T;
     double s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -209,7 +208,7 @@ __device__ __noinline__ double row_normaliser(const BeamArgs& A, int64_t row, fl
     if (A.history) {
         len = A.history_len ? A.history_len[row] : A.history_stride;
         len = max(0, min(len, A.history_stride));
-        for (int i = threadIdx.x; i < len; i += kThreads) sh.hist[i] = A.history[row * A.history_stride + i];
+        for (int i = threadIdx.x; i < len; i += kThreads) hist[i] = A.history[row * A.history_stride + i];
         __syncthreads();
     }
     const int chunk = A.history ? A.bit_words * 32 : A.V;
@@ -220,7 +219,7 @@ __device__ __noinline__ double row_normaliser(const BeamArgs& A, int64_t row, fl
             for (int i = threadIdx.x; i < A.bit_words; i += kThreads) bits[i] = 0;
             __syncthreads();
             for (int i = threadIdx.x; i < len; i += kThreads)
-                if (sh.hist[i] >= lo && sh.hist[i] < hi) atomicOr(&bits[(sh.hist[i] - lo) >> 5], 1u << ((sh.hist[i] - lo) & 31));
+                if (hist[i] >= lo && hist[i] < hi) atomicOr(&bits[(hist[i] - lo) >> 5], 1u << ((hist[i] - lo) & 31));
             __syncthreads();
         }
         // (eight loads in flight per thread, then their exponentials, into sums of their own)
@@ -238,12 +237,12 @@ __device__ __noinline__ double row_normaliser(const BeamArgs& A, int64_t row, fl
     }
     for (int i = threadIdx.x; i < len; i += kThreads) {
         // the first occurrence of a token: with its count
-        const int t = sh.hist[i];
+        const int t = hist[i];
         if (t < 0 || t >= A.V || !mask_bit(A, row, t)) continue;
         int n = 0;
         bool first = true;
         for (int j = 0; j < len; ++j) {
-            if (sh.hist[j] != t) continue;
+            if (hist[j] != t) continue;
             first = first && j >= i;
             ++n;
         }
@@ -539,7 +538,7 @@ __device__ __forceinline__ void extend_row(const BeamArgs& A, int b, double boun
 
 // The group's last CTA: merges the records, ranks, arranges, writes.
 template <typename T>
-__device__ __forceinline__ void finish_group(const BeamArgs& A, int n, BeamShared& sh, uint32_t* bits) {
+__device__ __forceinline__ void finish_group(const BeamArgs& A, int n, BeamShared& sh, uint32_t* bits, int32_t* hist) {
     const int K = A.K;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool done = A.done && A.done[n];
@@ -569,7 +568,7 @@ __device__ __forceinline__ void finish_group(const BeamArgs& A, int n, BeamShare
         for (int b = 0; b < K; ++b) {
             if (!((refine >> b) & 1u)) continue;
             const int64_t row = (int64_t)n * K + b;
-            const double l = row_normaliser<T>(A, row, sh.row_max[b], sh, bits);
+            const double l = row_normaliser<T>(A, row, sh.row_max[b], sh, bits, hist);
             if (tid == 0) sh.offset[b] = (double)A.scores[row] - l;
         }
         __syncthreads();
@@ -787,40 +786,43 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                                   ? logit_at<T>(reinterpret_cast<const T*>(A.logits) + G.row * A.row_stride + t) : -INFINITY;
             }
         }
-        // (the first copies behind the history's and the mask's reads, which would wait for them)
-        if (!started) {
-            started = true;
-            for (int i = 0; i < slots; ++i) issue_next();
-        }
         if constexpr (kBits) {
             __syncthreads();
             if (hist) {
                 // whoever clears a token's bit owns it; later occurrences are listed, to be counted; masked tokens are
                 // taken for later occurrences of nothing
                 const uint32_t bits0_at = smem_u32(bits);
-#pragma unroll 1
-                for (int g = 0; g < ns; ++g) {
-                    auto& G = sh.sg[g];
-                    const int o0 = (G.s0 - bits0) * kBlkTok - G.lo, len = G.n_own;
-                    int32_t* ids = own + g * A.hist_cap + tid;
-                    int32_t t[kIds];
-                    uint32_t was[kIds];
+                int32_t t[kBeamSegs][kIds];
+                uint32_t was[kBeamSegs][kIds];
+#pragma unroll
+                for (int g = 0; g < kBeamSegs; ++g) {
+                    const auto& G = sh.sg[g < ns ? g : 0];
+                    const int len = g < ns ? G.n_own : 0, o0 = (G.s0 - bits0) * kBlkTok - G.lo;
 #pragma unroll
                     for (int j = 0; j < kIds; ++j) {
-                        t[j] = tid + j * kThreads < len ? ids[j * kThreads] : -1;
-                        const int o = o0 + t[j];
-                        if (t[j] < G.lo || t[j] >= G.hi) t[j] = -1;
-                        else was[j] = smem_atom_and(bits0_at + (uint32_t)(o >> 5) * 4u, ~(1u << (o & 31))) >> (o & 31);
+                        t[g][j] = tid + j * kThreads < len ? own[g * A.hist_cap + tid + j * kThreads] : -1;
+                        const int o = o0 + t[g][j];
+                        if (t[g][j] < 0 || t[g][j] < G.lo || t[g][j] >= G.hi) t[g][j] = -1;
+                        else was[g][j] = smem_atom_and(bits0_at + (uint32_t)(o >> 5) * 4u, ~(1u << (o & 31))) >> (o & 31);
                     }
+                }
+#pragma unroll
+                for (int g = 0; g < kBeamSegs; ++g) {
 #pragma unroll
                     for (int j = 0; j < kIds; ++j) {
-                        const bool again = t[j] >= 0 && !(was[j] & 1u);
-                        if (again) dups[g * A.hist_cap + atomicAdd(&G.n_dups, 1)] = t[j];
-                        if (tid + j * kThreads < len && (again || t[j] < 0)) ids[j * kThreads] = -1;
+                        const bool again = t[g][j] >= 0 && !(was[g][j] & 1u);
+                        if (again) dups[g * A.hist_cap + atomicAdd(&sh.sg[g].n_dups, 1)] = t[g][j];
+                        if (again || t[g][j] < 0)
+                            if (tid + j * kThreads < A.hist_cap) own[g * A.hist_cap + tid + j * kThreads] = -1;
                     }
                 }
                 __syncthreads();
             }
+        }
+        // (the first copies behind the preparation, whose reads would wait for them)
+        if (!started) {
+            started = true;
+            for (int i = 0; i < slots; ++i) issue_next();
         }
 
         // ---- the stream: a lane has 32 consecutive tokens of a block
@@ -1102,7 +1104,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
 #pragma unroll 1
         for (int g = 0; g < ns; ++g) {
             if (sh.last[g] < 0) continue;
-            finish_group<T>(A, sh.last[g], sh, bits);
+            finish_group<T>(A, sh.last[g], sh, bits, own);
             __syncthreads();
         }
     }

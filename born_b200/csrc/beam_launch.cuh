@@ -6,7 +6,7 @@
 
 namespace born {
 
-constexpr int kBeamPiece = 128;     // blocks of a piece of a row: 16 KB of bits, 8 KB of group keys
+constexpr int kBeamPiece = 256;     // blocks of a piece of a row at most
 constexpr int kBeamMaxSlots = 8;    // ring slots of a warp
 
 // What a segment leaves for the merge.
