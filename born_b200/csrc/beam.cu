@@ -44,21 +44,28 @@ cudaError_t beam_attrs() {
     return e != cudaSuccess ? e : raise_limits<uint16_t>();
 }
 
-// A launch that may begin while the one before it ends (the kernels wait before they read).
+// A launch, in clusters of `cluster` CTAs, that may begin while the one before it ends (the kernels wait before they read).
 template <typename... P, typename... Q>
-static cudaError_t launch_after(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, const Q&... args) {
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
+static cudaError_t launch_clusters(int cluster, void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, const Q&... args) {
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3((unsigned)threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... P, typename... Q>
+static cudaError_t launch_after(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, const Q&... args) {
+    return launch_clusters(1, kernel, grid, threads, smem, st, args...);
 }
 
 template <typename T>
@@ -126,14 +133,20 @@ cudaError_t reorder_launch(ReorderArgs& A, cudaStream_t st) {
     return launch_after(reorder_kernel<uint8_t>, grid, kReorderThreads, 0, st, A);
 }
 
-constexpr int kSeqSmem = 222 * 1024;
+constexpr int kSeqSmem = 108 * 1024;  // two CTAs per SM
 cudaError_t sequences_attrs() { return cudaFuncSetAttribute(sequences_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSeqSmem); }
-cudaError_t sequences_launch(SequencesArgs& A, cudaStream_t st) {
+cudaError_t sequences_launch(SequencesArgs& A, int num_sms, cudaStream_t st) {
     A.shift = 2;
     while ((1 << A.shift) < A.K || (1 << A.shift) < A.H) ++A.shift;
-    A.tile = kSeqSmem / (6 << A.shift);  // a token and two bytes per beam
-    if (A.tile > A.T) A.tile = A.T;
-    return launch_after(sequences_kernel, (unsigned)A.N, kSeqThreads, (size_t)A.tile * (6 << A.shift), st, A);
+    A.ranks = 1;
+    // A cluster costs 1.5 us with two CTAs, 2.5 to 4 with four, and shares out the tables' bytes: 64 groups of 8 take 11 / 10 /
+    // 12 us for 1024 steps with one, two, four CTAs each, 38 / 25 / 20.5 us for 4096; one group of 4 8 / 8 / 9 and 21 / 14 / 11 us.
+    // Clusters that do not fit the GPU at once lose (256 groups, 1024 steps: 13 / 21 / 40 us).
+    while (A.ranks < kSeqRanks && A.ranks * A.N <= num_sms && A.T > A.ranks * 1024) A.ranks *= 2;
+    const int each = (A.T + A.ranks * kSeqChunks - 1) / (A.ranks * kSeqChunks) * kSeqChunks;
+    A.tile = kSeqSmem / (6 << A.shift) / kSeqChunks * kSeqChunks;  // a token and two bytes per beam
+    if (A.tile > each) A.tile = each;
+    return launch_clusters(A.ranks, sequences_kernel, (unsigned)(A.N * A.ranks), kSeqThreads, (size_t)A.tile * (6 << A.shift), st, A);
 }
 
 }  // namespace born

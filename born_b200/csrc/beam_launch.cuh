@@ -92,9 +92,10 @@ struct SequencesArgs {
     const int32_t *tokens, *parents, *end_step, *end_parent, *end_token;
     int32_t *out_tokens, *out_lens;
     int32_t pad;
-    int tile, shift;  // steps that shared memory holds at a time, 2^shift places each
+    int tile, shift;  // steps that a CTA's shared memory holds at a time, 2^shift places each
+    int ranks;        // CTAs of a group
 };
 cudaError_t sequences_attrs();
-cudaError_t sequences_launch(SequencesArgs& A, cudaStream_t st);
+cudaError_t sequences_launch(SequencesArgs& A, int num_sms, cudaStream_t st);
 
 }  // namespace born

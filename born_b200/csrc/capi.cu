@@ -1279,7 +1279,7 @@ int32_t born_beam_sequences(void* handle, const born_sequences_args* a, void* st
     A.tokens = a->tokens; A.parents = a->parents;
     A.end_step = a->end_step; A.end_parent = a->end_parent; A.end_token = a->end_token;
     A.out_tokens = a->out_tokens; A.out_lens = a->out_lens; A.pad = a->pad;
-    CUDA_TRY(h, sequences_launch(A, (cudaStream_t)stream));
+    CUDA_TRY(h, sequences_launch(A, h->num_sms, (cudaStream_t)stream));
     h->launches++;
     return BORN_OK;
 }

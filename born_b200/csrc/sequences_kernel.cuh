@@ -1,37 +1,43 @@
 // Sequences of hypotheses out of the tables that the steps of a beam search wrote.
 //
 // Following the parents back is a chain of dependent reads, one per step: 4096 steps would take a
-// millisecond of latency.  A step's parents are a map of at most 16 beams to 16 beams, and maps compose.  So a CTA
-// (one per group) brings parents and tokens of a tile of steps into shared memory, cuts the steps into 64 chunks, a
-// half warp each, and composes every chunk's map; a lane per hypothesis walks over the 64 maps; then all chunks
-// are walked at once, and the tokens are picked and written along the steps.  Longer tables go tile by
-// tile, from the end.
-// Bound by the bytes that one SM takes in (a group's rows are short pieces of the tables' rows) and by the two
-// walks, some 40 cycles a step: 64 groups of 8 beams, 4096 steps take 47 us when every chunk reads its own
-// parents and tokens as it walks, 36 us with the parents alone in shared memory.
+// millisecond of latency.  A step's parents are a map of at most 16 beams to 16 beams, and maps compose.  So a group's
+// CTAs (one, for long tables a cluster of two or four) bring parents and tokens of a tile of steps into shared memory, cut the
+// steps into 32 chunks each, a half warp per chunk, and compose every chunk's map; a lane per hypothesis walks over all
+// chunks' maps; then all chunks are walked at once, and the tokens are picked and written along the steps.  Longer
+// tables go tile by tile, from the end.
+// Bound by the short pieces that an SM takes in (a group's beams of each row of the tables) and by the walks, some 40
+// cycles a step: 64 groups of 8 beams and 4096 steps take 20.5 us (their bytes 3.9), 47 when every chunk reads its
+// own parents and tokens as it walks, 36 with the parents alone in shared memory, 26 with all of it in one CTA.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include "beam_launch.cuh"
+#include "scan_common.cuh"
 
 namespace born {
 
-constexpr int kSeqThreads = 1024;
-constexpr int kSeqChunks = kSeqThreads / 16;
+constexpr int kSeqThreads = 512;
+constexpr int kSeqChunks = kSeqThreads / 16;  // of a CTA
+constexpr int kSeqRanks = 4;                  // CTAs of a group at most
 constexpr uint32_t kNoLink = 0x80u;
 
-__global__ void __launch_bounds__(kSeqThreads) sequences_kernel(const SequencesArgs A) {
+__global__ void __launch_bounds__(kSeqThreads, 2) sequences_kernel(const SequencesArgs A) {
     extern __shared__ __align__(16) int32_t token_at[];  // [tile][width] tokens; then parents and beams, a byte each
-    __shared__ int8_t map[kSeqChunks][BORN_MAX_BEAMS];    // beam of a chunk's last step -> beam below its first
-    __shared__ int8_t entry[kSeqChunks][BORN_MAX_BEAMS];  // beam of hypothesis h at a chunk's last step
+    __shared__ __align__(16) int8_t map[kSeqRanks * kSeqChunks][BORN_MAX_BEAMS];  // beam of a chunk's last step -> beam below its first
+    __shared__ int8_t entry[kSeqRanks * kSeqChunks][BORN_MAX_BEAMS];  // beam of hypothesis h at a chunk's last step
     __shared__ int8_t low[BORN_MAX_BEAMS];                // ... below the chunk in which it ends
     __shared__ int8_t carry[BORN_MAX_BEAMS];              // ... at the last step of the tile that comes next
     __shared__ int ends[BORN_MAX_BEAMS];
     __shared__ int32_t last[BORN_MAX_BEAMS];
-    const int n = blockIdx.x, tid = threadIdx.x, chunk = tid >> 4, l = tid & 15;
+    const int R = A.ranks, n = (int)blockIdx.x / R, rank = (int)blockIdx.x % R;
+    const int tid = threadIdx.x, chunk = rank * kSeqChunks + (tid >> 4), l = tid & 15;
     const int K = A.K, T = A.T, H = A.H, shift = A.shift, W = 1 << shift;
     uint8_t* link = reinterpret_cast<uint8_t*>(token_at + A.tile * W);  // a step's parents; kNoLink: none
     uint8_t* beam = link + A.tile * W;                                  // beams of the hypotheses at a step
+    const int turn = 5 - shift;  // tokens of a step are turned round, so that a beam's are in different banks
+    __syncwarp();
+    cluster_arrive();  // (the others' shared memory is there)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int32_t* parents = A.parents + (int64_t)n * K;
@@ -49,9 +55,13 @@ __global__ void __launch_bounds__(kSeqThreads) sequences_kernel(const SequencesA
         ends[l] = e;
         carry[l] = 0;
     }
-    for (int tile = (T - 1) / A.tile; tile >= 0; --tile) {
-        const int base = tile * A.tile, steps = min(A.tile, T - base);
-        const int C = (steps + kSeqChunks - 1) / kSeqChunks, lo = chunk * C, hi = min(steps, lo + C);
+    bool first_tile = true;
+    for (int tile = (T - 1) / (A.tile * R); tile >= 0; --tile) {
+        // the cluster's steps base0 ..., of them this CTA's base ...; chunks in the cluster's numbers
+        const int base0 = tile * A.tile * R, all = min(A.tile * R, T - base0);
+        const int C = (all + kSeqChunks * R - 1) / (kSeqChunks * R), from = min(rank * kSeqChunks * C, all);
+        const int base = base0 + from, steps = min(kSeqChunks * C, all - from);
+        const int lo = (tid >> 4) * C, hi = min(steps, lo + C);
         // ---- the tables' rows; before step 0 a beam's parent is itself
         for (int i0 = tid; i0 < steps << shift; i0 += 8 * kSeqThreads) {
             int32_t p[8], v[8];
@@ -67,13 +77,15 @@ __global__ void __launch_bounds__(kSeqThreads) sequences_kernel(const SequencesA
                 const int i = i0 + u * kSeqThreads, t = i >> shift, b = i & (W - 1);
                 if (t >= steps) break;
                 link[i] = (uint8_t)(base + t == 0 ? b : p[u] < 0 || p[u] >= K ? kNoLink : p[u]);
-                token_at[i] = v[u];
+                token_at[(t << shift) + ((b + (t >> turn)) & (W - 1))] = v[u];
             }
         }
         __syncthreads();
+        if (first_tile) cluster_wait();
+        first_tile = false;
         // ---- the chunks' maps, and the hypotheses from their end to the bottom of its chunk
-        const int at = e - 1 - base;  // the hypothesis joins here
-        const bool joins = e > 0 && at >= 0 && at < steps;
+        const int at = e - 1 - base, at0 = e - 1 - base0;  // the hypothesis joins here
+        const bool joins = e > 0 && at0 >= 0 && at0 < all;
         {
             uint32_t r = l & (W - 1), b = 0, bad_r = 0, bad_b = 0;
             const uint8_t* row = link + (hi << shift);
@@ -91,23 +103,30 @@ __global__ void __launch_bounds__(kSeqThreads) sequences_kernel(const SequencesA
                 b &= 15u;
             }
             map[chunk][l] = (int8_t)(bad_r & kNoLink ? -1 : (int)r);
-            if (joins && at / C == chunk) low[l] = (int8_t)(bad_b & kNoLink ? -1 : (int)b);
+            if (joins && at0 / C == chunk)
+                for (int k = 0; k < R; ++k) *cluster_map(&low[l], k) = (int8_t)(bad_b & kNoLink ? -1 : (int)b);
         }
-        __syncthreads();
-        // ---- from chunk to chunk; a missing link empties the hypothesis
+        __syncwarp();
+        if (l < R && l != rank) *cluster_map(reinterpret_cast<uint4*>(map[chunk]), l) = *reinterpret_cast<const uint4*>(map[chunk]);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        // ---- from chunk to chunk; a missing link empties the hypothesis.  (A lane holds a map's entry for its beam and
+        // looks the beam it is at up in the others' registers: the maps are read ahead of the chain.)
         if (tid < 16) {
-            int c = -1, b = 0;
-            if (joins) {
-                c = at / C - 1;
-                b = low[l];
-            } else if (e - 1 >= base + steps) {
-                c = (steps - 1) / C;
-                b = carry[l];
+            const int top = (all - 1) / C;
+            const bool walks = joins || e - 1 >= base0 + all;
+            int c0 = -2, b = 0;  // where it starts: below chunk c0 + 1, at b
+            if (walks) {
+                c0 = joins ? at0 / C - 1 : top;
+                b = joins ? low[l] : carry[l];
             }
-            const bool walks = joins || c >= 0;
-            for (; c >= 0 && b >= 0; --c) {
+#pragma unroll 4
+            for (int c = top; c >= 0; --c) {
+                const int to = map[c][l];
                 entry[c][l] = (int8_t)b;
-                b = map[c][b];
+                const int below = __shfl_sync(0xffffu, to, b & 15, 16);
+                if (c <= c0 && b >= 0) b = below;
             }
             if (walks) {
                 carry[l] = (int8_t)max(b, 0);
@@ -132,13 +151,16 @@ __global__ void __launch_bounds__(kSeqThreads) sequences_kernel(const SequencesA
         for (int h = 0; h < H; ++h) {
             const int eh = ends[h] - base;
             for (int t = tid; t < steps; t += kSeqThreads)
-                out[h * A.out_stride + base + t] = t < eh ? token_at[(t << shift) + beam[(t << shift) + h]] : t == eh ? last[h] : A.pad;
+                out[h * A.out_stride + base + t] = t < eh ? token_at[(t << shift) + ((beam[(t << shift) + h] + (t >> turn)) & (W - 1))] : t == eh ? last[h] : A.pad;
         }
-        __syncthreads();
+        __syncwarp();
+        cluster_arrive();  // (maps that are still walked over; and nothing is written into a CTA that has ended)
+        cluster_wait();
     }
+    if (rank != 0) return;
     if (tid < H) A.out_lens[(int64_t)n * H + tid] = max(ends[tid], -1) + 1;
     // hypotheses whose missing link lay in an earlier tile than tokens already written
-    if (T > A.tile)
+    if (T > A.tile * R)
         for (int h = 0; h < H; ++h)
             if (ends[h] == -2)
                 for (int t = tid; t < T; t += kSeqThreads) out[h * A.out_stride + t] = A.pad;
