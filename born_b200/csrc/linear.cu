@@ -52,7 +52,7 @@ cudaError_t linear_attrs() {
 }
 
 template <typename O, int kCols, bool kPair, bool kTwo>
-static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, unsigned grid, cudaStream_t st) {
+static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& w1, const CUtensorMap& x, const LinearParams& P, unsigned grid, cudaStream_t st) {
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -67,20 +67,20 @@ static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& x, const Line
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = kPair ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair, kTwo>, w, x, P);
+    return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair, kTwo>, w, w1, x, P);
 }
 template <typename O>
-static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, bool pair, bool two, unsigned grid, cudaStream_t st) {
+static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& w1, const CUtensorMap& x, const LinearParams& P, bool pair, bool two, unsigned grid, cudaStream_t st) {
     if (two) {
-        if (pair) return launch<O, 128, true, true>(w, x, P, grid, st);
-        if (P.cols <= 16) return launch<O, 16, false, true>(w, x, P, grid, st);
-        return P.cols <= 32 ? launch<O, 32, false, true>(w, x, P, grid, st) : launch<O, 64, false, true>(w, x, P, grid, st);
+        if (pair) return launch<O, 128, true, true>(w, w1, x, P, grid, st);
+        if (P.cols <= 16) return launch<O, 16, false, true>(w, w1, x, P, grid, st);
+        return P.cols <= 32 ? launch<O, 32, false, true>(w, w1, x, P, grid, st) : launch<O, 64, false, true>(w, w1, x, P, grid, st);
     }
     const int cols = P.cols > 16 ? P.cols / 2 : 16;
-    if (pair) return cols <= 64 ? launch<O, 64, true, false>(w, x, P, grid, st) : launch<O, 128, true, false>(w, x, P, grid, st);
-    if (cols <= 16) return launch<O, 16, false, false>(w, x, P, grid, st);
-    if (cols <= 32) return launch<O, 32, false, false>(w, x, P, grid, st);
-    return cols <= 64 ? launch<O, 64, false, false>(w, x, P, grid, st) : launch<O, 128, false, false>(w, x, P, grid, st);
+    if (pair) return cols <= 64 ? launch<O, 64, true, false>(w, w1, x, P, grid, st) : launch<O, 128, true, false>(w, w1, x, P, grid, st);
+    if (cols <= 16) return launch<O, 16, false, false>(w, w1, x, P, grid, st);
+    if (cols <= 32) return launch<O, 32, false, false>(w, w1, x, P, grid, st);
+    return cols <= 64 ? launch<O, 64, false, false>(w, w1, x, P, grid, st) : launch<O, 128, false, false>(w, w1, x, P, grid, st);
 }
 
 cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStream_t st) {
@@ -101,15 +101,19 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStrea
     const bool pair = P.cols > 64 && A.V > kLinRows;
     const int unit_rows = pair ? 2 * kLinRows : kLinRows, room = pair ? num_sms / 2 : num_sms;
     const int x_rows = pair ? P.cols / 2 : P.cols;  // of the batch in a CTA
-    // Two tiles a CTA (up to 128 columns: tensor memory holds two accumulators of both) where that gives the
-    // busiest SM fewer rows to read, those of the batch included.  Hidden 4096, 128256 features, one tile -> two:
-    // 1 row 161 -> 173 us, 32 rows 184 -> 190, 64 rows 211 -> 194; 2048 x 32000 for 1 row 28.7 -> 24.9.
-    const auto busiest = [&](int rows) {
-        const int64_t units = (int64_t)((A.V + (int64_t)rows * (pair ? 2 : 1) - 1) / (rows * (pair ? 2 : 1))) * P.m_tiles;
-        return (units + room - 1) / room * (rows + x_rows);
-    };
-    const bool two = P.cols <= (pair ? 128 : 64) && busiest(2 * kLinRows) < busiest(kLinRows);
-    P.v_tiles = two ? (A.V + 2 * unit_rows - 1) / (2 * unit_rows) : (A.V + unit_rows - 1) / unit_rows;
+    // Two tiles a CTA for one slice of the batch (up to 128 columns: tensor memory holds two accumulators of both).  For pairs
+    // wherever a CTA has several tiles; where the busiest has an odd number, every CTA's last unit is a single one (one
+    // tile -> two, hidden 4096 and 128256 features: 100 rows 197 -> 188 us, 128 rows 202 -> 193; 8192 x 64000 for 128 rows 213 -> 189).
+    // CTAs on their own read few bytes of the batch and gain nothing (1 row of the first 161 -> 174, 64 rows 175 -> 178; 4096 x
+    // 37000, whose tiles fill their waves to 98%, 51.7 -> 52.5), except where an even number of waves of tiles leaves the GPU
+    // emptier than half as many of two (at 84%: 2048 x 32000 for 1 row 29 -> 25, 64 rows 30.6 -> 28.6; 8192 x 64000 182 -> 165, for 48 rows 192 -> 169).
+    const int singles = (A.V + unit_rows - 1) / unit_rows, each = (singles + room - 1) / room;
+    const bool two = P.m_tiles == 1 && each >= 2 && (pair ? P.cols <= 128 : P.cols <= 64 && each % 2 == 0 && (int64_t)singles * 10 < (int64_t)each * room * 9);
+    P.v_tiles = singles;
+    if (two) {
+        P.doubles = each % 2 ? each / 2 * room : (singles + 1) / 2;
+        P.v_tiles = P.doubles + (each % 2 ? singles - 2 * P.doubles : 0);
+    }
     // K is shared out while CTAs are left, in parts of four slices at least; adding up the parts costs the one that
     // does it their bytes, so wide tiles get few
     const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles;
@@ -131,12 +135,12 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStrea
     P.bias = A.bias; P.residual = A.residual; P.out = A.out;
     P.residual_stride = A.residual_stride; P.out_stride = A.out_stride;
     P.dev_error = A.dev_error; P.timeout_ns = A.timeout_ns;
-    CUtensorMap w, x;
-    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, w_rows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
+    CUtensorMap w, w1, x;
+    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, w_rows) || !make_map(&w1, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
     const int64_t units = tiles * P.splits;
     const unsigned grid = (unsigned)(units < room ? units : (int64_t)room) * (pair ? 2u : 1u);
-    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, x, P, pair, two, grid, st);
-    return launch_as<__nv_bfloat16>(w, x, P, pair, two, grid, st);
+    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, w1, x, P, pair, two, grid, st);
+    return launch_as<__nv_bfloat16>(w, w1, x, P, pair, two, grid, st);
 }
 
 }  // namespace born

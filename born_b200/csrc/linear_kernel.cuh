@@ -12,9 +12,9 @@
 // for every 128 rows of weights, and 256 columns of it twice the weights' bytes: out of L2, 256 rows of hidden
 // 4096 over 128256 features took 330 us with that.
 //
-// Up to 128 columns a CTA takes two such tiles at a time (kTwo), 256 v for one slice of the batch: L2 hands out some
-// 8.5 TB/s in all, and the batch's slices count as much as the weights there.  64 rows of hidden 4096, 128256
-// features: 209 us without.
+// Up to 128 columns a CTA takes two such tiles at a time (kTwo) where the launch finds that it pays, 256 v for one
+// slice of the batch: L2 hands out some 8.5 TB/s in all, and the batch's slices count as much as the weights there.  128
+// rows of hidden 4096, 128256 features take 193 us, 202 without (its bytes 171).
 //
 // The tensor core cuts partial sums off rather than rounding them, once per 16 products, which adds up: 4.3e-6 of
 // the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded.
@@ -22,9 +22,10 @@
 // Where the tiles are too few for the GPU, several CTAs (or pairs) share one, each with a part of K (splits).  They
 // leave their sums in scratch; the one that draws the tile's last ticket adds them up, in the order of the parts, and
 // finishes the tile.  No CTA waits for another one.  8192 x 1024 weights for one row: 45 us on the eight SMs that
-// have a tile, 12 us split.
+// have a tile, 15.5 us split.
 //
-// What bounds it: up to some 200 rows the bytes of the weights, beyond that the tensor pipe.
+// What bounds it: the bytes of the weights for few rows (1 row of the above: 161 us, the bytes' floor), then what L2 hands
+// out of weights and batch together (64 rows 175 us); 256 rows 244 us, 160 of them the tensor pipe's.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -50,6 +51,7 @@ struct LinearParams {
     int M, K, V;
     int cols;          // m of a tile
     int v_tiles, m_tiles;
+    int doubles;       // pairs in kTwo: so many units have two tiles a CTA, those behind them one
     int splits, part;  // CTAs (pairs) of a tile; slices of each
     float* partial;    // [tile of a CTA][split][cols][kLinRows]
     uint32_t* tickets; // [tile of a CTA]
@@ -206,7 +208,8 @@ __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __fl
 // of the tile's columns each, or the first one all 16; in kTwo a tile each).
 template <typename O, int kCols, bool kPair, bool kTwo>
 __global__ void __launch_bounds__(kLinThreads, 1)
-linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ LinearParams P) {
+linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wmap1, const __grid_constant__ CUtensorMap xmap,
+              const __grid_constant__ LinearParams P) {
     extern __shared__ uint8_t raw[];
     __shared__ LinearShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -218,6 +221,11 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     const int groups = kTwo || P.cols > 16 ? 2 : 1;          // of warps that take part in the epilogue
     constexpr int kMine = kTwo ? 2 * kLinRows : kLinRows;    // v of this CTA
     constexpr int kTileRows = kPair ? 2 * kMine : kMine;     // v of a unit
+    const auto is_double = [&](int u) { return kTwo && (!kPair || u < P.doubles); };
+    const auto first_v = [&](int u, int t) {  // of the unit in this CTA
+        if (!kTwo) return t / P.m_tiles * kTileRows + rank * kMine;
+        return is_double(u) ? u * kTileRows + rank * kMine : P.doubles * kTileRows + (u - P.doubles) * (kTileRows / 2) + rank * kLinRows;
+    };
     if (tid == 0) {
         for (int i = 0; i < P.stages; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -258,7 +266,9 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         bool ok = true;
         for (int u = first; u < units && ok; u += step) {
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
-            const int v0 = t / P.m_tiles * kTileRows + rank * kMine;
+            const int v0 = first_v(u, t);
+            const bool twice = is_double(u);
+            const int bytes = P.stage_bytes - (kTwo && !twice ? kLinRows * kLinK * 2 : 0);
             const int m0 = t % P.m_tiles * P.cols + (kPair ? rank * (P.cols / 2) : 0);
             for (int k = 0; k < slices; ++k) {
                 if (!lin_wait(sh, &sh.empty[stage], phase ^ 1u, P.timeout_ns)) {
@@ -267,8 +277,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 }
                 const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * P.stage_bytes);
                 if (rank == 0)
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(P.stage_bytes * (kPair ? 2 : 1)) : "memory");
-                tma_load_2d<kPair>(at, &wmap, (s0 + k) * kLinK, v0, bar);
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes * (kPair ? 2 : 1)) : "memory");
+                tma_load_2d<kPair>(at, kTwo && kPair && !twice ? &wmap1 : &wmap, (s0 + k) * kLinK, v0, bar);
                 tma_load_2d<kPair>(at + x_at, &xmap, (s0 + k) * kLinK, m0, bar);
                 ++issued;
                 if (++stage == P.stages) { stage = 0; phase ^= 1u; }
@@ -308,7 +318,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
 #pragma unroll
                     for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
-                    if constexpr (kTwo) {
+                    if (is_double(u)) {
                         const uint64_t a2 = smem_desc(at + kLinRows * kLinK * 2);
 #pragma unroll
                         for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
@@ -332,9 +342,10 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         bool ok = true;
         for (int u = first; u < units && ok; u += step) {
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
-            const int v = t / P.m_tiles * kTileRows + rank * kMine + r0, m0 = t % P.m_tiles * P.cols + c0;
+            const bool idle = kTwo && group && !is_double(u);
+            const int v = first_v(u, t) + r0, m0 = t % P.m_tiles * P.cols + c0;
             const int count = min(half, P.M - m0);  // (none for a group whose columns lie behind the batch)
-            const bool in = v < P.V;
+            const bool in = v < P.V && !idle;
             const float bias = P.bias && in ? P.bias[v] : 0.0f;
             float y[kCols];
             for (int k0 = 0; k0 < slices; k0 += kLinChunk, ++n) {
@@ -349,7 +360,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 const uint32_t d = d0 + (uint32_t)(acc * acc_cols);
 #pragma unroll
                 for (int c = 0; c < kCols; c += 16) {
-                    if (c >= half) break;
+                    if (c >= half || idle) break;
                     uint32_t r[16];
                     tmem_load16(d + (uint32_t)c, r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -401,6 +412,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 }
             }
             if (!ok) break;
+            if (idle) continue;
             O* out = reinterpret_cast<O*>(P.out) + (int64_t)m0 * P.out_stride + v;
             const O* res = reinterpret_cast<const O*>(P.residual) + (int64_t)m0 * P.residual_stride + v;
 #pragma unroll

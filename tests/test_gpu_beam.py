@@ -423,7 +423,7 @@ def test_reorder_past_32_bits(s):
 
 
 # ---- sequences ---------------------------------------------------------------------------------
-@pytest.mark.parametrize("N,K,T,H", [(1, 1, 1, 1), (2, 4, 2, 4), (3, 16, 255, 16), (1, 5, 256, 3), (2, 8, 257, 8), (4, 3, 1000, 5), (1, 16, 16384, 2), (1, 2, 70001, 2), (2, 4, 512, 4), (2, 4, 513, 4)])
+@pytest.mark.parametrize("N,K,T,H", [(1, 1, 1, 1), (2, 4, 2, 4), (3, 16, 255, 16), (1, 5, 256, 3), (2, 8, 257, 8), (4, 3, 1000, 5), (1, 16, 16384, 2), (1, 2, 70001, 2), (2, 4, 512, 4), (2, 4, 513, 4), (80, 4, 2049, 4), (3, 9, 5000, 2), (150, 2, 1500, 3)])
 @pytest.mark.parametrize("broken", [False, True])
 def test_sequences(s, N, K, T, H, broken):
     rng = np.random.default_rng(T)

@@ -32,7 +32,9 @@ def whole(shape, seed, lo=-2, hi=3):
 @pytest.mark.parametrize("M,K,V", [(1, 8, 1), (1, 16, 7), (2, 56, 127), (3, 64, 128), (15, 72, 129), (16, 128, 1000), (17, 1000, 515),
                                    (64, 512, 18944), (65, 136, 18945), (255, 264, 900), (256, 2048, 640), (257, 64, 300), (300, 192, 19100),
                                    (512, 320, 400), (700, 64, 257), (1, 8192, 300), (40, 4096, 40000),
-                                   (1, 8192, 1024), (16, 4104, 128), (33, 8000, 130), (128, 2048, 2000), (300, 3200, 1500), (512, 4096, 4096)])
+                                   (1, 8192, 1024), (16, 4104, 128), (33, 8000, 130), (128, 2048, 2000), (300, 3200, 1500), (512, 4096, 4096),
+                                   # two tiles a CTA: alone, in pairs, with single ones behind them
+                                   (9, 520, 32000), (50, 72, 32001), (128, 200, 37000), (100, 72, 45001), (70, 640, 80001)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_whole_numbers_are_exact(s, M, K, V, dtype):
     import torch
