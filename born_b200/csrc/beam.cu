@@ -114,6 +114,11 @@ cudaError_t beam_launch(BeamArgs& A, int dtype, bool aligned, int num_sms, cudaS
     return beam_launch_as<uint16_t>(A, has_bits, aligned, smem, st);
 }
 
+template <typename W>
+static cudaError_t reorder_launch_as(const ReorderArgs& A, unsigned grid, cudaStream_t st) {
+    if (A.K <= 4) return launch_after(reorder_kernel<W, 4>, grid, kReorderThreads, 0, st, A);
+    return launch_after(reorder_kernel<W, BORN_MAX_BEAMS>, grid, kReorderThreads, 0, st, A);
+}
 // The widest vectors that every row and piece is aligned to; ranges of 32 KB a CTA, smaller ones where
 // those would not fill the GPU.
 cudaError_t reorder_launch(ReorderArgs& A, cudaStream_t st) {
@@ -127,10 +132,10 @@ cudaError_t reorder_launch(ReorderArgs& A, cudaStream_t st) {
     while (pieces * ((piece + A.chunk - 1) / A.chunk) > 0x7fffffff) A.chunk *= 2;
     A.chunks = (int)((piece + A.chunk - 1) / A.chunk);
     const unsigned grid = (unsigned)(pieces * A.chunks);
-    if (low % 16 == 0) return launch_after(reorder_kernel<uint4>, grid, kReorderThreads, 0, st, A);
-    if (low % 4 == 0) return launch_after(reorder_kernel<uint32_t>, grid, kReorderThreads, 0, st, A);
-    if (low % 2 == 0) return launch_after(reorder_kernel<uint16_t>, grid, kReorderThreads, 0, st, A);
-    return launch_after(reorder_kernel<uint8_t>, grid, kReorderThreads, 0, st, A);
+    if (low % 16 == 0) return reorder_launch_as<uint4>(A, grid, st);
+    if (low % 4 == 0) return reorder_launch_as<uint32_t>(A, grid, st);
+    if (low % 2 == 0) return reorder_launch_as<uint16_t>(A, grid, st);
+    return reorder_launch_as<uint8_t>(A, grid, st);
 }
 
 constexpr int kSeqSmem = 108 * 1024;  // two CTAs per SM

@@ -38,8 +38,9 @@ __device__ __forceinline__ void move_bytes(uint8_t* base, int64_t row_stride, co
     }
 }
 
-template <typename W>
-__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderArgs A) {
+// kMost: beams of a group at most
+template <typename W, int kMost>
+__global__ void __launch_bounds__(kReorderThreads, kMost <= 4 ? 4 : 2) reorder_kernel(const __grid_constant__ ReorderArgs A) {
     __shared__ int dst[BORN_MAX_BEAMS], src[BORN_MAX_BEAMS];
     __shared__ int n_moves;
     // (chunk, piece, buffer, group), the chunks of a piece first
@@ -80,12 +81,12 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
     const int64_t count = bytes / (int64_t)sizeof(W);
     if (m == 1) move_bytes<W, 1>(base, A.row_stride, dst, src, m, count);
     else if (m == 2) move_bytes<W, 2>(base, A.row_stride, dst, src, m, count);
-    else if (m <= 4) move_bytes<W, 4>(base, A.row_stride, dst, src, m, count);
-    else if (m <= 8) move_bytes<W, 8>(base, A.row_stride, dst, src, m, count);
-    else move_bytes<W, 16>(base, A.row_stride, dst, src, m, count);
+    else if (kMost <= 4 || m <= 4) move_bytes<W, 4>(base, A.row_stride, dst, src, m, count);
+    else if (m <= 8) move_bytes<W, kMost <= 4 ? 4 : 8>(base, A.row_stride, dst, src, m, count);
+    else move_bytes<W, kMost <= 4 ? 4 : 16>(base, A.row_stride, dst, src, m, count);
     if constexpr (sizeof(W) > 1) {
         const int64_t rest = bytes - count * (int64_t)sizeof(W);
-        if (rest) move_bytes<uint8_t, 16>(base + count * (int64_t)sizeof(W), A.row_stride, dst, src, m, rest);
+        if (rest) move_bytes<uint8_t, kMost>(base + count * (int64_t)sizeof(W), A.row_stride, dst, src, m, rest);
     }
 }
 
