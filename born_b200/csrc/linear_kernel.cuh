@@ -415,15 +415,23 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             if (idle) continue;
             O* out = reinterpret_cast<O*>(P.out) + (int64_t)m0 * P.out_stride + v;
             const O* res = reinterpret_cast<const O*>(P.residual) + (int64_t)m0 * P.residual_stride + v;
+            if (P.bias) {
 #pragma unroll
-            for (int c = 0; c < kCols; c += 16) {
-                if (c >= count) break;
-                if (P.bias) {
+                for (int c = 0; c < kCols; ++c) y[c] += bias;
+            }
+            if (P.activation == BORN_ACT_NONE && !P.residual) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) y[c + i] += bias;
+                for (int c = 0; c < kCols; ++c) {
+                    if (in && c < count) store_out(out, y[c]);
+                    out += P.out_stride;
                 }
-                activate(P, y + c);
-                // (an address at a time: 128 of them would not fit the registers)
+                continue;
+            }
+            // (16 columns at a time, those behind them moved up: with all 128 unrolled the code does not stay in the
+            // instruction cache: of 256 rows of 128256 features gelu took 110 us instead of 30, tanh 26 instead of 18)
+#pragma unroll 1
+            for (int c = 0; c < count; c += 16) {
+                activate(P, y);
                 if (P.residual) {
                     float r[16];
 #pragma unroll
@@ -432,13 +440,15 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                         res += P.residual_stride;
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) y[c + i] += r[i];
+                    for (int i = 0; i < 16; ++i) y[i] += r[i];
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    if (in && c + i < count) store_out(out, y[c + i]);
+                    if (in && c + i < count) store_out(out, y[i]);
                     out += P.out_stride;
                 }
+#pragma unroll
+                for (int i = 0; i + 16 < kCols; ++i) y[i] = y[i + 16];
             }
         }
     }
