@@ -55,6 +55,9 @@ class BeamSearch:
         self.scores = torch.empty(rows, dtype=torch.float32, device=dev)
         self.status = torch.empty(rows, **i32)
         self.pool = sampler.beam_pool(self.groups, self.beams)
+        # (held here: the kernel writes them after the step's call has returned, on whatever stream it was given)
+        self.ends = {n: torch.empty((self.groups, self.beams), dtype=d, device=dev) for n, d in
+                     (("end_parent", torch.int32), ("end_token", torch.int32), ("end_score", torch.float32))}
         self.logits = torch.empty((rows, self.vocab), dtype=torch.float32, device=dev) if head is not None else None
         self.steps = None
         if self.history:
@@ -101,13 +104,16 @@ class BeamSearch:
             logits = s.linear(x, h.weight, bias=h.bias, activation=h.activation, scale=h.scale, out=self.logits, stream=stream)
         if tuple(logits.shape) != (self.groups * self.beams, self.vocab):
             raise InvalidArgument(f"logits are {tuple(logits.shape)}, not {(self.groups * self.beams, self.vocab)}")
+        states = list(states)
+        moves = [s.prepare_beam_reorder(part, self.parent_table[t], self.beams, lens=lens, position_dim=position_dim)
+                 for part in (states if states and isinstance(states[0], (list, tuple)) else [states] if states else [])]
         make = s.beam_next if self.history else s.beam_step
         make(logits, self.scores, self.beams, config=self.config, mask=mask, pool=self.pool, step=t, stream=stream,
-             out={"token": self.token_table[t], "parent": self.parent_table[t], "score": self.scores, "status": self.status})
+             out={"token": self.token_table[t], "parent": self.parent_table[t], "score": self.scores, "status": self.status,
+                  **self.ends})
         self.steps = t + 1
-        states = list(states)
-        for part in (states if states and isinstance(states[0], (list, tuple)) else [states] if states else []):
-            s.beam_reorder(part, self.parent_table[t], self.beams, lens=lens, position_dim=position_dim, stream=stream)
+        for move in moves:
+            move.run(stream)
         return self.token_table[t]
 
     def result(self, stream=None):
@@ -117,6 +123,7 @@ class BeamSearch:
         if not self.steps:
             raise InvalidArgument("no step has been made")
         N, K, T, p = self.groups, self.beams, self.steps, self.pool
+        i32 = dict(dtype=torch.int32, device=self.scores.device)
         with self._on(stream):
             going = (p.done == 0)[:, None] & (self.tokens.view(N, K) >= 0)
             score = torch.where(going, self.scores.view(N, K) / float(T) ** C.c_float(self.config.length_penalty).value, -math.inf)
@@ -125,5 +132,6 @@ class BeamSearch:
             last = torch.where(going, T - 1, -1).to(torch.int32)
             ends = [torch.cat(pair, 1).gather(1, order).contiguous() for pair in
                     ((p.step, last), (p.parent, self.parent_table[T - 1].view(N, K)), (p.token, self.tokens.view(N, K)))]
-        out = self.sampler.beam_sequences(self.token_table[:T], self.parent_table[:T], *ends, K, stream=stream)
+            out = {"tokens": torch.empty((N, K, T), **i32), "lens": torch.empty((N, K), **i32)}
+        self.sampler.beam_sequences(self.token_table[:T], self.parent_table[:T], *ends, K, out=out, stream=stream)
         return {"tokens": out["tokens"], "lens": out["lens"], "scores": scores}

@@ -87,7 +87,7 @@ cudaError_t beam_launch(BeamArgs& A, int dtype, bool aligned, int num_sms, cudaS
     for (int most = kBeamPiece;; most = most * 3 / 4 > kBeamLeastPiece ? most * 3 / 4 : kBeamLeastPiece) {
         row_pieces(A.V, most, A.pieces, A.pb);
         const int64_t pieces = (int64_t)A.N * A.K * A.pieces, blocks = pieces * A.pb;
-        if (blocks > 0x7fffffff / kBlkTok) return cudaErrorInvalidValue;
+        if (blocks > (int64_t)(0xffffffffu / (2u * (unsigned)num_sms))) return cudaErrorNotSupported;  // (range_start, record_of: 32 bits)
         A.blocks = (int)blocks;
         // a block per warp at least, a CTA of its own for every piece while the GPU holds them at once
         int64_t grid = (blocks + kBeamWarps - 1) / kBeamWarps;

@@ -71,6 +71,7 @@ struct BeamArgs {
 int64_t beam_max_records(int max_batch, int max_vocab, int num_sms);
 cudaError_t beam_attrs();
 // Fills in how the rows are dealt; cudaErrorInvalidValue where they are too many.
+// cudaErrorNotSupported: more rows than the numbering of the blocks holds
 cudaError_t beam_launch(BeamArgs& A, int dtype, bool aligned, int num_sms, cudaStream_t st);
 
 // ---- born_beam_reorder ------------------------------------------------------------------------

@@ -1169,7 +1169,9 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
         A.ring_cap = h->ring_cap;
     }
     const bool aligned = rows_aligned(1, a->vocab, a->logits_dtype, a->logits, rows > 1 ? a->logits_row_stride : 0);
-    CUDA_TRY(h, beam_launch(A, a->logits_dtype, aligned, h->num_sms, st));
+    const cudaError_t e = beam_launch(A, a->logits_dtype, aligned, h->num_sms, st);
+    if (e == cudaErrorNotSupported) return fail(h, BORN_ERR_UNSUPPORTED, "beam_step: %lld rows of %d tokens are too many for one call", (long long)rows, a->vocab);
+    CUDA_TRY(h, e);
     h->launches++;
     return BORN_OK;
 }
@@ -1246,6 +1248,8 @@ int32_t born_beam_reorder(void* handle, const born_reorder_args* a, void* stream
     memset(&A, 0, sizeof A);
     for (int i = 0; i < a->n_buffers; ++i) {
         if (!a->buffers[i]) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: buffer %d is NULL", i);
+        for (int j = 0; j < i; ++j)
+            if (a->buffers[i] == a->buffers[j]) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: buffers %d and %d are the same", j, i);
         A.buffers[i] = (uint8_t*)a->buffers[i];
     }
     if (a->beams == 1) return BORN_OK;
@@ -1266,6 +1270,7 @@ int32_t born_beam_sequences(void* handle, const born_sequences_args* a, void* st
     int rc = args_check(h, a, "beam_sequences");
     if (rc || (rc = groups_check(h, a->groups, a->beams, "beam_sequences"))) return rc;
     if (a->steps < 1 || a->hypotheses < 1) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_sequences: steps and hypotheses must be positive");
+    if (a->steps > 1 << 30) return fail(h, BORN_ERR_UNSUPPORTED, "beam_sequences: %d steps exceed %d", a->steps, 1 << 30);
     if (a->hypotheses > BORN_MAX_BEAMS) return fail(h, BORN_ERR_UNSUPPORTED, "beam_sequences: %d hypotheses exceed %d", a->hypotheses, BORN_MAX_BEAMS);
     if (a->table_stride < (int64_t)a->groups * a->beams || a->out_stride < a->steps)
         return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_sequences: table_stride < groups x beams, or out_stride < steps");
@@ -1292,9 +1297,11 @@ int32_t born_linear(void* handle, const born_linear_args* a, void* stream) {
     if (rc) return rc;
     if (a->rows < 1 || a->hidden < 1 || a->features < 1)
         return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: rows %d, hidden %d and features %d must be positive", a->rows, a->hidden, a->features);
+    if (a->rows > kLinMost || a->hidden > kLinMost || a->features > kLinMost)
+        return fail(h, BORN_ERR_UNSUPPORTED, "linear: rows %d, hidden %d and features %d: at most %d", a->rows, a->hidden, a->features, kLinMost);
     if (a->out_dtype != BORN_DTYPE_F32 && a->out_dtype != BORN_DTYPE_BF16) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: unknown out_dtype %d", a->out_dtype);
     if (a->activation < BORN_ACT_NONE || a->activation > BORN_ACT_SILU) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: unknown activation %d", a->activation);
-    if (!(a->scale >= 0.0f) || !isfinite(a->scale)) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: scale out of range");
+    if (!(a->scale >= 0.0f) || !isfinite(a->scale) || (a->scale != 0.0f && !isnormal(a->scale))) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: scale out of range");
     if (!a->x || !a->weight || !a->out) return fail(h, BORN_ERR_INVALID_ARGUMENT, "linear: x, weight and out are required");
     if (a->x_row_stride < a->hidden || a->weight_row_stride < a->hidden || a->out_row_stride < a->features ||
         (a->residual && a->residual_row_stride < a->features))

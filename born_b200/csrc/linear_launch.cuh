@@ -6,6 +6,8 @@
 
 namespace born {
 
+constexpr int kLinMost = 0x7fffffff - 1024;  // rows, hidden, features: a tile further is still an int
+
 struct LinearArgs {
     int M, K, V;
     int activation;

@@ -390,7 +390,8 @@ int32_t born_beam_pool_reset(void* handle, const born_beam_args* args, void* str
 /* Arguments of born_beam_reorder: in every buffer, row n*beams + b becomes what row
  * n*beams + parents[n*beams + b] was, in place; a parent outside 0..beams-1 leaves the row as it is.
  * A row is `planes` pieces (heads, layers) of `positions` positions of position_bytes contiguous
- * bytes; only the first lens[n] positions move, what lies behind them stays.  Buffers must not overlap. */
+ * bytes; only the first lens[n] positions move, what lies behind them stays.  Rows of different buffers must
+ * not overlap (a buffer given twice is refused). */
 typedef struct born_reorder_args {
     uint32_t struct_size;
     uint32_t memory; /* BORN_MEM_DEVICE: the buffers, parents, lens; `buffers` itself is a host array */
@@ -455,7 +456,7 @@ typedef struct born_linear_args {
     int32_t features;  /* v */
     int32_t out_dtype; /* BORN_DTYPE_* of out and residual */
     int32_t activation; /* BORN_ACT_* */
-    float scale;        /* BORN_ACT_TANH: > 0 (0 => 1) */
+    float scale;        /* BORN_ACT_TANH: > 0, no subnormal (0 => 1) */
     const void* x;           /* [rows, x_row_stride] bf16 */
     const void* weight;      /* [features, weight_row_stride] bf16 */
     const float* bias;       /* [features] fp32; NULL = none */

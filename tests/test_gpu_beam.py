@@ -715,3 +715,72 @@ def test_search_refusals(s):
     b.step(z)
     with pytest.raises(InvalidArgument):
         b.step(z)
+
+
+def test_search_steps_allocate_nothing(s):
+    """What a step writes must not be memory that the caller's other work gets while the kernel still runs."""
+    import torch
+    from born_b200 import BeamConfig, BeamSearch
+    N, K, V = 2, 4, 600
+    z = torch.randn((N * K, V), device="cuda")
+    state = torch.zeros((N * K, 8), device="cuda")
+    search = BeamSearch(s, N, K, 6, V, BeamConfig(stop_tokens=(3,)))
+    search.begin()
+    search.step(z, states=[state])
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    for _ in range(5):
+        search.step(z, states=[state])
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+
+
+def test_search_refuses_states_before_the_step(s):
+    import torch
+    from born_b200 import BeamSearch, InvalidArgument
+    N, K, V = 2, 4, 600
+    z = torch.randn((N * K, V), device="cuda")
+    search = BeamSearch(s, N, K, 6, V)
+    search.begin()
+    scores = search.scores.clone()
+    with pytest.raises(InvalidArgument):
+        search.step(z, states=[torch.zeros((N * K + 1, 8), device="cuda")])
+    assert search.steps == 0 and torch.equal(search.scores, scores)
+
+
+def test_sizes_that_are_refused(s):
+    import torch
+    from born_b200 import InvalidArgument, SamplerError, _lib as L
+    i32 = dict(dtype=torch.int32, device="cuda")
+    p, z = torch.zeros(8, **i32), torch.zeros((8, 100), device="cuda")
+    with pytest.raises(InvalidArgument):  # rows would be moved twice at once
+        s.beam_reorder([z, torch.zeros_like(z), z], p, 4)
+    t, e = torch.zeros((5, 8), **i32), torch.zeros((2, 4), **i32)
+    call = s.prepare_beam_sequences(t, t, e, e, e, 4)
+    call.args.steps = call.args.out_stride = 2 ** 30 + 1
+    with pytest.raises(SamplerError) as err:
+        call.run()
+    assert err.value.code == L.ERR_UNSUPPORTED
+
+
+def test_thousands_of_groups(lib):
+    """More rows than 2^31 tokens hold; every row has its best tokens at places of its own."""
+    import torch
+    from born_b200 import Sampler
+    N, K, V = 2200, 8, 131072
+    R = N * K
+    z = torch.zeros((R, V), dtype=torch.bfloat16, device="cuda")
+    at = torch.arange(R, device="cuda") * 7919 % (V - 8)
+    for j in range(K):
+        z[torch.arange(R, device="cuda"), at + j] = 12.0 - j
+    scores = torch.full((R,), -math.inf, device="cuda")
+    scores[::K] = 0.0
+    with Sampler(device=0, max_batch=R, max_vocab=V) as big:
+        out = big.beam_step(z, scores, K)
+        want = at[::K, None] + torch.arange(K, device="cuda")
+        assert torch.equal(out["token"].view(N, K).long(), want)
+        assert (out["parent"] == 0).all()
+        # All beams alive and alike in score: the best token of each.  In which order is open: the rows hold the same values
+        # in different places, so their normalisers are equal but for the rounding of a sum in another order.
+        out = big.beam_step(z, torch.zeros(R, device="cuda"), K)
+        parent = out["parent"].view(N, K).long()
+        assert torch.equal(parent.sort(1).values, torch.arange(K, device="cuda").expand(N, K))
+        assert torch.equal(out["token"].view(N, K).long(), at.view(N, K).gather(1, parent))

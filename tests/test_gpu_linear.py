@@ -207,3 +207,18 @@ def test_refusals(s):
         setattr(call.args, field, value)
         bad(*err, call.run)
         setattr(call.args, field, keep)
+
+
+def test_sizes_that_are_refused(s):
+    from born_b200 import InvalidArgument, SamplerError, _lib as L
+    call = s.prepare_linear(whole((4, 64), 1), whole((100, 64), 2), activation="tanh")
+    for field in ("rows", "hidden", "features"):
+        keep = getattr(call.args, field)
+        setattr(call.args, field, 2 ** 31 - 1000)
+        with pytest.raises(SamplerError) as e:
+            call.run()
+        assert e.value.code == L.ERR_UNSUPPORTED
+        setattr(call.args, field, keep)
+    call.args.scale = 1e-40  # whose inverse is no number
+    with pytest.raises(InvalidArgument):
+        call.run()
