@@ -77,9 +77,7 @@ struct Handle {
     BeamRecord* beam_records = nullptr;
     int64_t beam_records_cap = 0;
     uint32_t* beam_tickets = nullptr;
-    // output head: sums of tiles whose K several CTAs share, and a ticket per tile
-    float* linear_partial = nullptr;
-    uint32_t* linear_ticket = nullptr;
+    LinearLimits linear_limits = {};
     // grammar-mask upload (born_mask_*)
     uint32_t* mask_host[2] = {nullptr, nullptr};
     uint32_t* mask_dev[2] = {nullptr, nullptr};
@@ -346,7 +344,6 @@ int check_device_error(Handle* h) {
         // tickets of rows that were left unfinished must not leak into the next launch
         cudaMemset(h->tickets, 0, sizeof(uint32_t) * 2 * (size_t)h->max_rows);
         if (h->beam_tickets) cudaMemset(h->beam_tickets, 0, sizeof(uint32_t) * (size_t)h->max_batch);
-        if (h->linear_ticket) cudaMemset(h->linear_ticket, 0, sizeof(uint32_t) * (size_t)linear_tickets(h->num_sms));
         cudaMemset(h->dev_error, 0, sizeof(int));
         return fail(h, BORN_ERR_DEVICE_TIMEOUT, "a bounded on-device wait gave up (code %d); outputs of that call are invalid", e);
     }
@@ -435,16 +432,13 @@ int32_t born_sampler_create(int32_t device, int32_t max_batch, int32_t max_vocab
     h->beam_records_cap = beam_max_records(max_batch, max_vocab, h->num_sms);
     if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->beam_records, (size_t)h->beam_records_cap * sizeof(BeamRecord));
     if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->beam_tickets, sizeof(uint32_t) * (size_t)max_batch);
-    if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->linear_partial, (size_t)linear_scratch_bytes(h->num_sms));
-    if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->linear_ticket, sizeof(uint32_t) * (size_t)linear_tickets(h->num_sms));
-    if (rc == BORN_OK && cudaMemset(h->linear_ticket, 0, sizeof(uint32_t) * (size_t)linear_tickets(h->num_sms)) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cudaMemset(h->beam_tickets, 0, sizeof(uint32_t) * (size_t)max_batch) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cudaMemset(h->tickets, 0, sp.tickets) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cudaMemset(h->dev_error, 0, 32 * sizeof(int)) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && scan_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cluster_limits(h->max_clusters) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && spec_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
-    if (rc == BORN_OK && (beam_attrs() != cudaSuccess || sequences_attrs() != cudaSuccess || linear_attrs() != cudaSuccess)) rc = BORN_ERR_CUDA;
+    if (rc == BORN_OK && (beam_attrs() != cudaSuccess || sequences_attrs() != cudaSuccess || linear_attrs(h->linear_limits) != cudaSuccess)) rc = BORN_ERR_CUDA;
     for (int i = 0; i < 4 && rc == BORN_OK; ++i)
         if (cudaEventCreate(&h->ev[i]) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc != BORN_OK) {
@@ -474,8 +468,6 @@ int32_t born_sampler_destroy(void* handle) {
     cudaFree(h->tickets);
     cudaFree(h->seg_packed);
     cudaFree(h->dev_error);
-    cudaFree(h->linear_partial);
-    cudaFree(h->linear_ticket);
     cudaFree(h->beam_records);
     cudaFree(h->beam_tickets);
     cudaFree(h->spec_scratch);
@@ -1322,11 +1314,9 @@ int32_t born_linear(void* handle, const born_linear_args* a, void* stream) {
     A.x = a->x; A.weight = a->weight; A.bias = a->bias; A.residual = a->residual; A.out = a->out;
     A.x_stride = a->x_row_stride; A.weight_stride = a->weight_row_stride;
     A.residual_stride = a->residual_row_stride; A.out_stride = a->out_row_stride;
-    A.partial = h->linear_partial;
-    A.tickets = h->linear_ticket;
     A.dev_error = h->dev_error;
     A.timeout_ns = h->timeout_ns;
-    CUDA_TRY(h, linear_launch(A, a->out_dtype, h->num_sms, (cudaStream_t)stream));
+    CUDA_TRY(h, linear_launch(A, a->out_dtype, h->num_sms, h->linear_limits, (cudaStream_t)stream));
     h->launches++;
     return BORN_OK;
 }

@@ -44,11 +44,24 @@ static cudaError_t raise_limits() {
         if (x != cudaSuccess) return x;
     return cudaSuccess;
 }
-int64_t linear_scratch_bytes(int num_sms) { return (int64_t)num_sms * kLinSplitCols * kLinRows * 4; }
-int linear_tickets(int num_sms) { return num_sms; }
-cudaError_t linear_attrs() {
-    const cudaError_t e = raise_limits<float>();
-    return e != cudaSuccess ? e : raise_limits<__nv_bfloat16>();
+cudaError_t linear_attrs(LinearLimits& limits) {
+    cudaError_t e = raise_limits<float>();
+    if (e == cudaSuccess) e = raise_limits<__nv_bfloat16>();
+    for (int n = 2; n <= kLinMaxCluster && e == cudaSuccess; ++n) {
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = (unsigned)n;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof cfg);
+        cfg.gridDim = dim3((unsigned)n, 1, 1);
+        cfg.blockDim = dim3(kLinThreads, 1, 1);
+        cfg.dynamicSmemBytes = kLinSmem;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&limits.clusters[n], linear_kernel<float, 64, false, false>, &cfg);
+    }
+    return e;
 }
 
 template <typename O, int kCols, bool kPair, bool kTwo>
@@ -57,7 +70,7 @@ static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& w1, const CUt
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = kPair ? 2 : 1;
+    at[1].val.clusterDim.x = (unsigned)(P.splits * (kPair ? 2 : 1));
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
@@ -66,7 +79,7 @@ static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& w1, const CUt
     cfg.dynamicSmemBytes = (size_t)P.stages * P.stage_bytes + 1024;
     cfg.stream = st;
     cfg.attrs = at;
-    cfg.numAttrs = kPair ? 2 : 1;
+    cfg.numAttrs = kPair || P.splits > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair, kTwo>, w, w1, x, P);
 }
 template <typename O>
@@ -83,7 +96,7 @@ static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& w1, const 
     return cols <= 64 ? launch<O, 64, false, false>(w, w1, x, P, grid, st) : launch<O, 128, false, false>(w, w1, x, P, grid, st);
 }
 
-cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStream_t st) {
+cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, const LinearLimits& limits, cudaStream_t st) {
     LinearParams P;
     memset(&P, 0, sizeof P);
     P.M = A.M; P.K = A.K; P.V = A.V;
@@ -114,17 +127,17 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStrea
         P.doubles = each % 2 ? each / 2 * room : (singles + 1) / 2;
         P.v_tiles = P.doubles + (each % 2 ? singles - 2 * P.doubles : 0);
     }
-    // K is shared out while CTAs are left, in parts of four slices at least; adding up the parts costs the one that
-    // does it their bytes, so wide tiles get few
+    // K is shared out while CTAs are left, in parts of four slices at least, over the CTAs of a cluster (8 at most: larger ones
+    // are not portable).
     const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles;
     const int slices = (A.K + kLinK - 1) / kLinK;
     int64_t splits = room / tiles;
     if (splits > slices / 4) splits = slices / 4;
-    if (splits > 1024 / P.cols) splits = 1024 / P.cols;
+    if (splits > kLinMaxCluster / (pair ? 2 : 1)) splits = kLinMaxCluster / (pair ? 2 : 1);
+    while (splits > 1 && limits.clusters[splits * (pair ? 2 : 1)] < tiles) --splits;  // (all at once: 16 of 8 do not fit 148 SMs)
     if (splits < 1 || two || P.cols > kLinSplitCols) splits = 1;
     P.part = (int)((slices + splits - 1) / splits);
     P.splits = (slices + P.part - 1) / P.part;
-    P.partial = A.partial; P.tickets = A.tickets;
     const int w_rows = two ? 2 * kLinRows : kLinRows;
     P.stage_bytes = (w_rows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
     P.stages = (kLinSmem - 1024) / P.stage_bytes;

@@ -19,10 +19,9 @@
 // The tensor core cuts partial sums off rather than rounding them, once per 16 products, which adds up: 4.3e-6 of
 // the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded.
 //
-// Where the tiles are too few for the GPU, several CTAs (or pairs) share one, each with a part of K (splits).  They
-// leave their sums in scratch; the one that draws the tile's last ticket adds them up, in the order of the parts, and
-// finishes the tile.  No CTA waits for another one.  8192 x 1024 weights for one row: 45 us on the eight SMs that
-// have a tile, 15.5 us split.
+// Where the tiles are too few for the GPU, the CTAs (or pairs) of a cluster share one, each with a part of K (splits).  They
+// leave their sums in the place of their rings; every CTA adds up a share of the columns out of all of them, in the
+// order of the parts, and finishes those.  @@
 //
 // What bounds it: the bytes of the weights for few rows (1 row of the above: 161 us, the bytes' floor), then what L2 hands
 // out of weights and batch together (64 rows 175 us); 256 rows 244 us, 160 of them the tensor pipe's.
@@ -42,7 +41,7 @@ constexpr int kLinRows = 128;      // v of a CTA's tile
 constexpr int kLinK = 64;          // elements of a slice: 128 bytes, one swizzle atom
 constexpr int kLinChunk = 8;       // slices that the tensor core sums
 constexpr int kLinMaxCols = 256;   // m of a tile
-constexpr int kLinSplitCols = 128; // ... where K is shared out (the scratch is sized for it)
+constexpr int kLinSplitCols = 128; // ... where K is shared out
 constexpr int kLinMaxStages = 12;
 constexpr int kLinThreads = 384;   // warps: 0 TMA, 1 products, 2 tensor memory, 3 idle, 4..11 epilogue
 constexpr int kLinSmem = 220 * 1024;
@@ -53,8 +52,6 @@ struct LinearParams {
     int v_tiles, m_tiles;
     int doubles;       // pairs in kTwo: so many units have two tiles a CTA, those behind them one
     int splits, part;  // CTAs (pairs) of a tile; slices of each
-    float* partial;    // [tile of a CTA][split][cols][kLinRows]
-    uint32_t* tickets; // [tile of a CTA]
     int stages, stage_bytes, tmem_cols;  // of a CTA
     int activation;
     float scale, inv_scale;
@@ -70,7 +67,6 @@ struct LinearShared {
     uint64_t full[kLinMaxStages], empty[kLinMaxStages];
     uint64_t acc_full[2], acc_empty[2], drained;
     uint32_t tmem;
-    int last;
     volatile int failed;
 };
 
@@ -131,12 +127,23 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
             "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
             : "memory");
 }
-// An arrival, once the products issued so far are done, at the barrier (of both CTAs in kPair).
+// Shared memory of the cluster's CTA `rank`, at the place that `at` is in this one.
+__device__ __forceinline__ uint32_t remote_smem(uint32_t at, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float load_remote(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+// pair: rank of the pair's first CTA in the cluster.  An arrival, once the products issued so far are done, at the barrier (of both CTAs in kPair).
 template <bool kPair>
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t pair) {
     if constexpr (kPair)
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-                     "h"((uint16_t)3)
+                     "h"((uint16_t)(3u << pair))
                      : "memory");
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -144,23 +151,9 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 // An arrival at the barrier of the pair's first CTA.  What it orders are reads of tensor memory that tcgen05.wait::ld has
 // seen done; a release to the whole cluster would wait for the output's stores as well (128 rows of hidden 1024, 151936
 // features 73.6 -> 70.1 us without, 256 rows of hidden 4096, 128256 features with tanh 265 -> 257.5).
-__device__ __forceinline__ void arrive_first(uint64_t* bar) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+__device__ __forceinline__ void arrive_first(uint64_t* bar, uint32_t pair) {
+    const uint32_t a = remote_smem(smem_u32(bar), (int)pair);
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
-}
-// Barrier of the epilogue's threads: whether any of them says so.
-__device__ __forceinline__ bool epilogue_any(bool pred, int threads) {
-    int r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.s32 p, %1, 0;\n\t"
-        "bar.red.or.pred q, 1, %2, p;\n\t"
-        "selp.s32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"((int)pred), "r"(threads)
-        : "memory");
-    return r != 0;
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -175,27 +168,28 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
         : "r"(addr));
 }
 
-__device__ __forceinline__ void activate(const LinearParams& P, float* v) {
+template <int N>
+__device__ __forceinline__ void activate(const LinearParams& P, float (&v)[N]) {
     switch (P.activation) {
         case BORN_ACT_RELU:
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
+            for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
             break;
         case BORN_ACT_SIGMOID:
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 1.0f / (1.0f + expf(-v[i]));
+            for (int i = 0; i < N; ++i) v[i] = 1.0f / (1.0f + expf(-v[i]));
             break;
         case BORN_ACT_TANH:
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = P.scale * tanhf(v[i] * P.inv_scale);
+            for (int i = 0; i < N; ++i) v[i] = P.scale * tanhf(v[i] * P.inv_scale);
             break;
         case BORN_ACT_GELU:
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * (float)M_SQRT1_2));
+            for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * (float)M_SQRT1_2));
             break;
         case BORN_ACT_SILU:
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = v[i] / (1.0f + expf(-v[i]));
+            for (int i = 0; i < N; ++i) v[i] = v[i] / (1.0f + expf(-v[i]));
             break;
         default: break;
     }
@@ -217,6 +211,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;  // swizzle atoms start on 1024 bytes
     const int rank = kPair ? (int)(blockIdx.x & 1u) : 0;     // in the pair
+    const uint32_t pair = kPair ? (blockIdx.x & ~1u) % (2u * (uint32_t)P.splits) : 0;  // its first CTA's rank in the cluster
+    float* sums = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));
     const int first = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int units = P.v_tiles * P.m_tiles * P.splits;      // tiles, times the parts of K
     const int all_slices = (P.K + kLinK - 1) / kLinK;
@@ -325,14 +321,14 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
 #pragma unroll
                         for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
                     }
-                    mma_commit<kPair>(&sh.empty[stage]);
+                    mma_commit<kPair>(&sh.empty[stage], pair);
                     if (++stage == P.stages) { stage = 0; phase ^= 1u; }
                 }
-                if (ok) mma_commit<kPair>(&sh.acc_full[acc]);
+                if (ok) mma_commit<kPair>(&sh.acc_full[acc], pair);
             }
         }
         // tensor memory is given back only after the last product (bounded, like the copies)
-        mma_commit<kPair>(&sh.drained);
+        mma_commit<kPair>(&sh.drained, pair);
         lin_settle(smem_u32(&sh.drained), 0, P.timeout_ns);
     } else if (warp >= 4 && (warp - 4) >> 2 < groups) {
         // ---- epilogue
@@ -377,41 +373,16 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    if constexpr (kPair) arrive_first(&sh.acc_empty[acc]);
+                    if constexpr (kPair) arrive_first(&sh.acc_empty[acc], pair);
                     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.acc_empty[acc])) : "memory");
                 }
             }
-            if (!kTwo && P.splits > 1) {
-                const int mine = kPair ? 2 * t + rank : t, row = r0;
-                float* tile = P.partial + (int64_t)mine * P.splits * P.cols * kLinRows + (int64_t)c0 * kLinRows + row;
-                float* to = tile + (int64_t)(u - t * P.splits) * P.cols * kLinRows;
+            if (!kTwo && P.splits > 1) {  // (every slice has been used up: the sums take the ring's place)
+                float* to = sums + c0 * kLinRows + r0;
 #pragma unroll
                 for (int c = 0; c < kCols; ++c)
-                    if (ok && c < half) __stcg(to + c * kLinRows, y[c]);
-                // (a warp whose wait ran out takes the others along: none is left waiting at a barrier)
-                if (epilogue_any(!ok, 128 * groups)) ok = false;
-                if (!ok) break;
-                if (tid == 128) {
-                    __threadfence();
-                    const bool last = atomicAdd(&P.tickets[mine], 1u) == (uint32_t)P.splits - 1u;
-                    if (last) {
-                        P.tickets[mine] = 0;
-                        __threadfence();
-                    }
-                    sh.last = last;
-                }
-                asm volatile("bar.sync 1, %0;" ::"r"(128 * groups) : "memory");
-                const bool last = sh.last;
-                asm volatile("bar.sync 1, %0;" ::"r"(128 * groups) : "memory");  // (read by all before the next unit's is written)
-                if (!last) continue;
-#pragma unroll
-                for (int c = 0; c < kCols; ++c) y[c] = 0.0f;
-                for (int s = 0; s < P.splits; ++s) {
-                    const float* from = tile + (int64_t)s * P.cols * kLinRows;
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c)
-                        if (c < half) y[c] += __ldcg(from + c * kLinRows);
-                }
+                    if (c < half) to[c * kLinRows] = y[c];
+                continue;
             }
             if (!ok) break;
             if (idle) continue;
@@ -433,7 +404,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             // instruction cache: of 256 rows of 128256 features gelu took 110 us and tanh 26, now 23 and 12)
 #pragma unroll 1
             for (int c = 0; c < count; c += 16) {
-                activate(P, y);
+                activate(P, reinterpret_cast<float(&)[16]>(y));
                 if (P.residual) {
                     float r[16];
 #pragma unroll
@@ -455,6 +426,35 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         }
     }
     __syncwarp();
+    if (!kTwo && P.splits > 1) {
+        // ---- the parts of K: a CTA of the cluster adds up its share of the columns and finishes them
+        cluster_sync();
+        const int S = P.splits, t = first / S, row = tid % kLinRows, v = first_v(first, t) + row, m0 = t % P.m_tiles * P.cols;
+        const int cols = min(P.cols, P.M - m0), stride = kLinThreads / kLinRows * S;
+        const float bias = P.bias && v < P.V ? P.bias[v] : 0.0f;
+        for (int c = first % S + tid / kLinRows * S; c < cols; c += 4 * stride) {
+            float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for (int s = 0; s < S; ++s) {
+                const uint32_t from = remote_smem(ring + (uint32_t)((c * kLinRows + row) * 4), kPair ? 2 * s + rank : s);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j * stride < cols) z[j] += load_remote(from + (uint32_t)(j * stride * kLinRows * 4));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[j] += bias;
+            activate(P, z);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int m = m0 + c + j * stride;
+                if (c + j * stride >= cols || v >= P.V) break;
+                if (P.residual) z[j] += load_out(reinterpret_cast<const O*>(P.residual) + (int64_t)m * P.residual_stride + v);
+                store_out(reinterpret_cast<O*>(P.out) + (int64_t)m * P.out_stride + v, z[j]);
+            }
+        }
+        __syncwarp();
+        if constexpr (!kPair) cluster_sync();  // (the others have read this CTA's sums)
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if constexpr (kPair) cluster_sync();

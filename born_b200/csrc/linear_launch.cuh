@@ -8,6 +8,11 @@ namespace born {
 
 constexpr int kLinMost = 0x7fffffff - 1024;  // rows, hidden, features: a tile further is still an int
 
+constexpr int kLinMaxCluster = 8;  // larger clusters are not portable
+struct LinearLimits {
+    int clusters[kLinMaxCluster + 1];  // so many of 2, 3, ... CTAs run at once
+};
+
 struct LinearArgs {
     int M, K, V;
     int activation;
@@ -18,16 +23,11 @@ struct LinearArgs {
     const void* residual;
     void* out;
     int64_t x_stride, weight_stride, residual_stride, out_stride;  // elements
-    // scratch for tiles whose K several CTAs share: their sums, and tickets that are 0 between launches
-    float* partial;
-    uint32_t* tickets;
     int* dev_error;
     unsigned long long timeout_ns;
 };
-int64_t linear_scratch_bytes(int num_sms);
-int linear_tickets(int num_sms);
-cudaError_t linear_attrs();
+cudaError_t linear_attrs(LinearLimits& limits);
 // dtype: of out and residual
-cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, cudaStream_t st);
+cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, const LinearLimits& limits, cudaStream_t st);
 
 }  // namespace born
