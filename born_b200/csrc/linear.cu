@@ -96,64 +96,85 @@ static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& w1, const 
     return cols <= 64 ? launch<O, 64, false, false>(w, w1, x, P, grid, st) : launch<O, 128, false, false>(w, w1, x, P, grid, st);
 }
 
-cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, const LinearLimits& limits, cudaStream_t st) {
-    LinearParams P;
-    memset(&P, 0, sizeof P);
-    P.M = A.M; P.K = A.K; P.V = A.V;
-    P.v_tiles = (A.V + kLinRows - 1) / kLinRows;
-    // As few column tiles as hold the rows, of equal widths; narrower ones where the tiles are few (rows x hidden x
-    // features with 256, 128, 64 columns: 128 x 4096 x 4096 27.4, 27.3, 20.2 us; 256 x 8192 x 2000 53, 32, 31;
-    // 512 x 4096 x 4096 31, 29, 37, whose tiles of 64 columns are more than the SMs).
-    int most = kLinMaxCols;
-    if ((int64_t)P.v_tiles * ((A.M + most - 1) / most) * 2 <= num_sms) most = (int64_t)P.v_tiles * ((A.M + 63) / 64) <= num_sms ? 64 : kLinSplitCols;
-    P.m_tiles = (A.M + most - 1) / most;
+// How a product is cut: the tiles, who shares what, and what that costs.
+struct LinearShape {
+    int cols, m_tiles, v_tiles, doubles, splits, part;
+    bool pair, two;
+    int64_t cost;  // nanoseconds, about: see below
+};
+// ... with tiles of `most` columns at most
+static LinearShape shape_of(const LinearArgs& A, int most, int num_sms, const LinearLimits& limits) {
+    LinearShape S;
+    // as few column tiles as hold the rows, of equal widths
+    S.m_tiles = (A.M + most - 1) / most;
     const int unit = A.M <= 16 ? 16 : 32;  // (a multiple of 16 for either half of the epilogue)
-    P.cols = ((A.M + P.m_tiles - 1) / P.m_tiles + unit - 1) / unit * unit;
-    P.m_tiles = (A.M + P.cols - 1) / P.cols;
+    S.cols = ((A.M + S.m_tiles - 1) / S.m_tiles + unit - 1) / unit * unit;
+    S.m_tiles = (A.M + S.cols - 1) / S.cols;
     // A pair from 65 columns on: below that the batch's slices are a third of the bytes at most
-    const bool pair = P.cols > 64 && A.V > kLinRows;
-    const int unit_rows = pair ? 2 * kLinRows : kLinRows, room = pair ? num_sms / 2 : num_sms;
-    const int x_rows = pair ? P.cols / 2 : P.cols;  // of the batch in a CTA
+    S.pair = S.cols > 64 && A.V > kLinRows;
+    const int ctas = S.pair ? 2 : 1, unit_rows = ctas * kLinRows, room = num_sms / ctas, x_rows = S.cols / ctas;
     // Two tiles a CTA for one slice of the batch (up to 128 columns: tensor memory holds two accumulators of both).  For pairs
     // wherever a CTA has several tiles; where the busiest has an odd number, every CTA's last unit is a single one (one
     // tile -> two, hidden 4096 and 128256 features: 100 rows 197 -> 188 us, 128 rows 202 -> 193; 8192 x 64000 for 128 rows 213 -> 189).
     // CTAs on their own read few bytes of the batch and gain nothing (1 row of the first 161 -> 174, 64 rows 175 -> 178; 4096 x
     // 37000, whose tiles fill their waves to 98%, 51.7 -> 52.5), except where an even number of waves of tiles leaves the GPU
     // emptier than half as many of two (at 84%: 2048 x 32000 for 1 row 29 -> 25, 64 rows 30.6 -> 28.6; 8192 x 64000 182 -> 165, for 48 rows 192 -> 169).
-    const int singles = (A.V + unit_rows - 1) / unit_rows, each = (singles + room - 1) / room;
-    const bool two = P.m_tiles == 1 && each >= 2 && (pair ? P.cols <= 128 : P.cols <= 64 && each % 2 == 0 && (int64_t)singles * 10 < (int64_t)each * room * 9);
-    P.v_tiles = singles;
-    if (two) {
-        P.doubles = each % 2 ? each / 2 * room : (singles + 1) / 2;
-        P.v_tiles = P.doubles + (each % 2 ? singles - 2 * P.doubles : 0);
+    const int singles = (A.V + unit_rows - 1) / unit_rows;
+    int64_t each = ((int64_t)singles * S.m_tiles + room - 1) / room;
+    S.two = S.m_tiles == 1 && each >= 2 && (S.pair ? S.cols <= 128 : S.cols <= 64 && each % 2 == 0 && (int64_t)singles * 10 < each * room * 9);
+    S.v_tiles = singles;
+    S.doubles = 0;
+    if (S.two) {
+        S.doubles = each % 2 ? (int)(each / 2) * room : (singles + 1) / 2;
+        S.v_tiles = S.doubles + (each % 2 ? singles - 2 * S.doubles : 0);
     }
-    // K is shared out while CTAs are left, in parts of four slices at least, over the CTAs of a cluster (8 at most: larger ones
-    // are not portable).
-    const int64_t tiles = (int64_t)P.v_tiles * P.m_tiles;
+    // K is shared out while CTAs are left, in parts of four slices at least, over the CTAs of a cluster, and so that all
+    // clusters run at once (16 of 8 CTAs do not: 1 x 2048 x 2048 11.3 us with those, 6.8 with 16 of 7).
+    const int64_t tiles = (int64_t)S.v_tiles * S.m_tiles;
     const int slices = (A.K + kLinK - 1) / kLinK;
     int64_t splits = room / tiles;
     if (splits > slices / 4) splits = slices / 4;
-    if (splits > kLinMaxCluster / (pair ? 2 : 1)) splits = kLinMaxCluster / (pair ? 2 : 1);
-    while (splits > 1 && limits.clusters[splits * (pair ? 2 : 1)] < tiles) --splits;  // (all at once: 16 of 8 do not fit 148 SMs)
-    if (splits < 1 || two || P.cols > kLinSplitCols) splits = 1;
-    P.part = (int)((slices + splits - 1) / splits);
-    P.splits = (slices + P.part - 1) / P.part;
-    const int w_rows = two ? 2 * kLinRows : kLinRows;
+    if (splits > kLinMaxCluster / ctas) splits = kLinMaxCluster / ctas;
+    while (splits > 1 && limits.clusters[splits * ctas] < tiles) --splits;
+    if (splits < 1 || S.two) splits = 1;
+    S.part = (int)((slices + splits - 1) / splits);
+    S.splits = (slices + S.part - 1) / S.part;
+    // The busiest CTA: 2 ns for 64 elements of a row, of weights or batch; per tile 15 ns a column for the epilogue's end; the
+    // joining of parts 1.5 us and 7 ns a column.  (Fitted to 16 shapes of 80 to 512 rows, within 2 us.)
+    const int64_t reads = S.two ? each / 2 * (2 * kLinRows + x_rows) + each % 2 * (kLinRows + x_rows) : each * (kLinRows + x_rows);
+    S.cost = 2 * S.part * reads + 15 * each * S.cols + (S.splits > 1 ? 1500 + 7 * S.cols : 0);
+    return S;
+}
+
+cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, const LinearLimits& limits, cudaStream_t st) {
+    // Wide tiles read the weights once, narrow ones fill the GPU and have less of an end.  Rows x hidden x features with
+    // 256, 128, 64 columns: 256 x 512 x 4096 13.1, 9.8, 6.2 us; 512 x 4096 x 1000 17.2, 15.7, 17.8; 512 x 4096 x 4096 25.9, 29.1, 48.
+    LinearShape S = shape_of(A, kLinMaxCols, num_sms, limits);
+    for (int most = kLinMaxCols / 2; most >= 64 && A.M > 64; most /= 2) {
+        const LinearShape o = shape_of(A, most, num_sms, limits);
+        if (o.cost < S.cost) S = o;
+    }
+    LinearParams P;
+    memset(&P, 0, sizeof P);
+    P.M = A.M; P.K = A.K; P.V = A.V;
+    P.cols = S.cols; P.m_tiles = S.m_tiles; P.v_tiles = S.v_tiles; P.doubles = S.doubles;
+    P.splits = S.splits; P.part = S.part;
+    const int w_rows = S.two ? 2 * kLinRows : kLinRows, x_rows = S.pair ? S.cols / 2 : S.cols;
     P.stage_bytes = (w_rows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
     P.stages = (kLinSmem - 1024) / P.stage_bytes;
     if (P.stages > kLinMaxStages) P.stages = kLinMaxStages;
     P.tmem_cols = 32;
-    while (P.tmem_cols < (two ? 4 : 2) * P.cols) P.tmem_cols *= 2;
+    while (P.tmem_cols < (S.two ? 4 : 2) * P.cols) P.tmem_cols *= 2;
     P.activation = A.activation; P.scale = A.scale; P.inv_scale = 1.0f / A.scale;
     P.bias = A.bias; P.residual = A.residual; P.out = A.out;
     P.residual_stride = A.residual_stride; P.out_stride = A.out_stride;
     P.dev_error = A.dev_error; P.timeout_ns = A.timeout_ns;
     CUtensorMap w, w1, x;
     if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, w_rows) || !make_map(&w1, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
-    const int64_t units = tiles * P.splits;
-    const unsigned grid = (unsigned)(units < room ? units : (int64_t)room) * (pair ? 2u : 1u);
-    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, w1, x, P, pair, two, grid, st);
-    return launch_as<__nv_bfloat16>(w, w1, x, P, pair, two, grid, st);
+    const int64_t units = (int64_t)P.v_tiles * P.m_tiles * P.splits, room = S.pair ? num_sms / 2 : num_sms;
+    const unsigned grid = (unsigned)(units < room ? units : room) * (S.pair ? 2u : 1u);
+    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, w1, x, P, S.pair, S.two, grid, st);
+    return launch_as<__nv_bfloat16>(w, w1, x, P, S.pair, S.two, grid, st);
 }
 
 }  // namespace born

@@ -34,7 +34,10 @@ def whole(shape, seed, lo=-2, hi=3):
                                    (512, 320, 400), (700, 64, 257), (1, 8192, 300), (40, 4096, 40000),
                                    (1, 8192, 1024), (16, 4104, 128), (33, 8000, 130), (128, 2048, 2000), (300, 3200, 1500), (512, 4096, 4096),
                                    # two tiles a CTA: alone, in pairs, with single ones behind them
-                                   (9, 520, 32000), (50, 72, 32001), (128, 200, 37000), (100, 72, 45001), (70, 640, 80001)])
+                                   (9, 520, 32000), (50, 72, 32001), (128, 200, 37000), (100, 72, 45001), (70, 640, 80001),
+                                   # K over clusters of two to eight, tiles of every width, lone CTAs of 256 columns
+                                   (200, 2048, 1000), (256, 8192, 2001), (130, 1032, 3001), (512, 4104, 1001), (256, 520, 4096), (150, 4096, 100),
+                                   (256, 2048, 128), (8, 2048, 513), (128, 4096, 1024), (1, 2048, 2048), (1, 520, 1)])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_whole_numbers_are_exact(s, M, K, V, dtype):
     import torch
