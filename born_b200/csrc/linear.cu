@@ -76,7 +76,7 @@ static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& w1, const CUt
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3(kLinThreads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)P.stages * P.stage_bytes + 1024;
+    cfg.dynamicSmemBytes = (size_t)P.stages * lin_deep(kTwo) * P.slice_bytes + 1024;
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = kPair || P.splits > 1 ? 2 : 1;
@@ -160,8 +160,8 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, const Lin
     P.cols = S.cols; P.m_tiles = S.m_tiles; P.v_tiles = S.v_tiles; P.doubles = S.doubles;
     P.splits = S.splits; P.part = S.part;
     const int w_rows = S.two ? 2 * kLinRows : kLinRows, x_rows = S.pair ? S.cols / 2 : S.cols;
-    P.stage_bytes = (w_rows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
-    P.stages = (kLinSmem - 1024) / P.stage_bytes;
+    P.slice_bytes = (w_rows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
+    P.stages = (kLinSmem - 1024) / (lin_deep(S.two) * P.slice_bytes);
     if (P.stages > kLinMaxStages) P.stages = kLinMaxStages;
     P.tmem_cols = 32;
     while (P.tmem_cols < (S.two ? 4 : 2) * P.cols) P.tmem_cols *= 2;

@@ -43,6 +43,7 @@ constexpr int kLinK = 64;          // elements of a slice: 128 bytes, one swizzl
 constexpr int kLinChunk = 8;       // slices that the tensor core sums
 constexpr int kLinMaxCols = 256;   // m of a tile
 constexpr int kLinMaxStages = 12;
+__host__ __device__ constexpr int lin_deep(bool two) { return two ? 1 : 2; }  // slices of a ring stage
 constexpr int kLinThreads = 384;   // warps: 0 TMA, 1 products, 2 tensor memory, 3 idle, 4..11 epilogue
 constexpr int kLinSmem = 220 * 1024;
 
@@ -52,7 +53,7 @@ struct LinearParams {
     int v_tiles, m_tiles;
     int doubles;       // pairs in kTwo: so many units have two tiles a CTA, those behind them one
     int splits, part;  // CTAs (pairs) of a tile; slices of each
-    int stages, stage_bytes, tmem_cols;  // of a CTA
+    int stages, slice_bytes, tmem_cols;  // of a CTA
     int activation;
     float scale, inv_scale;
     const float* bias;
@@ -219,6 +220,8 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     const int groups = kTwo || P.cols > 16 ? 2 : 1;          // of warps that take part in the epilogue
     constexpr int kMine = kTwo ? 2 * kLinRows : kLinRows;    // v of this CTA
     constexpr int kTileRows = kPair ? 2 * kMine : kMine;     // v of a unit
+    constexpr int kDeep = lin_deep(kTwo);
+    const int stage_bytes = kDeep * P.slice_bytes;
     const auto is_double = [&](int u) { return kTwo && (!kPair || u < P.doubles); };
     const auto first_v = [&](int u, int t) {  // of the unit in this CTA
         if (!kTwo) return t / P.m_tiles * kTileRows + rank * kMine;
@@ -266,18 +269,24 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
             const int v0 = first_v(u, t);
             const bool twice = is_double(u);
-            const int bytes = P.stage_bytes - (kTwo && !twice ? kLinRows * kLinK * 2 : 0);
+            const int bytes = P.slice_bytes - (kTwo && !twice ? kLinRows * kLinK * 2 : 0);
             const int m0 = t % P.m_tiles * P.cols + (kPair ? rank * (P.cols / 2) : 0);
-            for (int k = 0; k < slices; ++k) {
+            for (int k = 0; k < slices; k += kDeep) {
                 if (!lin_wait(sh, &sh.empty[stage], phase ^ 1u, P.timeout_ns)) {
                     ok = false;
                     break;
                 }
-                const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * P.stage_bytes);
+                const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * stage_bytes);
+                const int n = min(kDeep, slices - k);
                 if (rank == 0)
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes * (kPair ? 2 : 1)) : "memory");
-                tma_load_2d<kPair>(at, kTwo && kPair && !twice ? &wmap1 : &wmap, (s0 + k) * kLinK, v0, bar);
-                tma_load_2d<kPair>(at + x_at, &xmap, (s0 + k) * kLinK, m0, bar);
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * bytes * (kPair ? 2 : 1)) : "memory");
+#pragma unroll
+                for (int j = 0; j < kDeep; ++j) {
+                    if (j >= n) break;
+                    const uint32_t to = at + (uint32_t)(j * P.slice_bytes);
+                    tma_load_2d<kPair>(to, kTwo && kPair && !twice ? &wmap1 : &wmap, (s0 + k + j) * kLinK, v0, bar);
+                    tma_load_2d<kPair>(to + x_at, &xmap, (s0 + k + j) * kLinK, m0, bar);
+                }
                 ++issued;
                 if (++stage == P.stages) { stage = 0; phase ^= 1u; }
             }
@@ -306,20 +315,24 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + (uint32_t)(acc * acc_cols);
                 const int k1 = min(slices, k0 + kLinChunk);
-                for (int k = k0; k < k1; ++k) {
+                for (int k = k0; k < k1; k += kDeep) {
                     if (!lin_wait(sh, &sh.full[stage], phase, P.timeout_ns)) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = ring + (uint32_t)(stage * P.stage_bytes);
-                    const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
 #pragma unroll
-                    for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
-                    if (is_double(u)) {
-                        const uint64_t a2 = smem_desc(at + kLinRows * kLinK * 2);
+                    for (int j = 0; j < kDeep; ++j) {
+                        if (k + j >= k1) break;
+                        const uint32_t at = ring + (uint32_t)(stage * stage_bytes + j * P.slice_bytes);
+                        const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
 #pragma unroll
-                        for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k - k0) | i));
+                        for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
+                        if (is_double(u)) {
+                            const uint64_t a2 = smem_desc(at + kLinRows * kLinK * 2);
+#pragma unroll
+                            for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
+                        }
                     }
                     mma_commit<kPair>(&sh.empty[stage], pair);
                     if (++stage == P.stages) { stage = 0; phase ^= 1u; }
