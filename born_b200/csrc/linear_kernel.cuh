@@ -95,6 +95,15 @@ __device__ __forceinline__ void lin_settle(uint32_t bar, uint32_t parity, unsign
         if ((it & 15u) == 15u && global_timer_ns() - t0 > limit_ns) break;
 }
 
+__device__ __forceinline__ bool elected() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
 // K-major operand with the 128-byte swizzle: groups of 8 rows 1024 bytes apart.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -209,7 +218,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
               const __grid_constant__ LinearParams P) {
     extern __shared__ uint8_t raw[];
     __shared__ LinearShared sh;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (known to be uniform)
     const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;  // swizzle atoms start on 1024 bytes
     const int rank = kPair ? (int)(blockIdx.x & 1u) : 0;     // in the pair
     const uint32_t pair = kPair ? (blockIdx.x & ~1u) % (2u * (uint32_t)P.splits) : 0;  // its first CTA's rank in the cluster
@@ -298,8 +307,9 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             if (--stage < 0) { stage = P.stages - 1; phase ^= 1u; }
             lin_settle(smem_u32(&sh.full[stage]), phase, P.timeout_ns);
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // ---- products: D fp32, A and B bf16, both K-major
+    } else if (warp == 1 && rank == 0) {
+        // ---- products: D fp32, A and B bf16, both K-major.  The whole warp goes along, one lane issues.
+        const bool issues = elected();
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(P.cols >> 3) << 17) | ((uint32_t)((kPair ? 2 * kLinRows : kLinRows) >> 4) << 24);
         int stage = 0, n = 0;
         uint32_t phase = 0;
@@ -308,7 +318,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
             for (int k0 = 0; k0 < slices && ok; k0 += kLinChunk, ++n) {
                 const int acc = n & 1;
-                if (!lin_wait(sh, &sh.acc_empty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, P.timeout_ns)) {
+                if (!__all_sync(0xffffffffu, lin_wait(sh, &sh.acc_empty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, P.timeout_ns))) {
                     ok = false;
                     break;
                 }
@@ -316,32 +326,36 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 const uint32_t d = tmem + (uint32_t)(acc * acc_cols);
                 const int k1 = min(slices, k0 + kLinChunk);
                 for (int k = k0; k < k1; k += kDeep) {
-                    if (!lin_wait(sh, &sh.full[stage], phase, P.timeout_ns)) {
+                    if (!__all_sync(0xffffffffu, lin_wait(sh, &sh.full[stage], phase, P.timeout_ns))) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (issues) {
 #pragma unroll
-                    for (int j = 0; j < kDeep; ++j) {
-                        if (k + j >= k1) break;
-                        const uint32_t at = ring + (uint32_t)(stage * stage_bytes + j * P.slice_bytes);
-                        const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
+                        for (int j = 0; j < kDeep; ++j) {
+                            if (k + j >= k1) break;
+                            const uint32_t at = ring + (uint32_t)(stage * stage_bytes + j * P.slice_bytes);
+                            const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
 #pragma unroll
-                        for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
-                        if (is_double(u)) {
-                            const uint64_t a2 = smem_desc(at + kLinRows * kLinK * 2);
+                            for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
+                            if (is_double(u)) {
+                                const uint64_t a2 = smem_desc(at + kLinRows * kLinK * 2);
 #pragma unroll
-                            for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
+                                for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
+                            }
                         }
+                        mma_commit<kPair>(&sh.empty[stage], pair);
                     }
-                    mma_commit<kPair>(&sh.empty[stage], pair);
+                    __syncwarp();
                     if (++stage == P.stages) { stage = 0; phase ^= 1u; }
                 }
-                if (ok) mma_commit<kPair>(&sh.acc_full[acc], pair);
+                if (ok && issues) mma_commit<kPair>(&sh.acc_full[acc], pair);
+                __syncwarp();
             }
         }
         // tensor memory is given back only after the last product (bounded, like the copies)
-        mma_commit<kPair>(&sh.drained, pair);
+        if (issues) mma_commit<kPair>(&sh.drained, pair);
         lin_settle(smem_u32(&sh.drained), 0, P.timeout_ns);
     } else if (warp >= 4 && (warp - 4) >> 2 < groups) {
         // ---- epilogue
