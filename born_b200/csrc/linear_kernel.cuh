@@ -268,8 +268,9 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    if (warp == 0 && lane == 0) {
-        // ---- producer: this CTA's rows of weights, its share of the batch's
+    if (warp == 0) {
+        // ---- producer: this CTA's rows of weights, its share of the batch's.  (The whole warp, like the products'.)
+        const bool issues = elected();
         int stage = 0;
         uint32_t phase = 0;
         long long issued = 0;
@@ -281,21 +282,24 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
             const int bytes = P.slice_bytes - (kTwo && !twice ? kLinRows * kLinK * 2 : 0);
             const int m0 = t % P.m_tiles * P.cols + (kPair ? rank * (P.cols / 2) : 0);
             for (int k = 0; k < slices; k += kDeep) {
-                if (!lin_wait(sh, &sh.empty[stage], phase ^ 1u, P.timeout_ns)) {
+                if (!__all_sync(0xffffffffu, lin_wait(sh, &sh.empty[stage], phase ^ 1u, P.timeout_ns))) {
                     ok = false;
                     break;
                 }
                 const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * stage_bytes);
                 const int n = min(kDeep, slices - k);
-                if (rank == 0)
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * bytes * (kPair ? 2 : 1)) : "memory");
+                if (issues) {
+                    if (rank == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * bytes * (kPair ? 2 : 1)) : "memory");
 #pragma unroll
-                for (int j = 0; j < kDeep; ++j) {
-                    if (j >= n) break;
-                    const uint32_t to = at + (uint32_t)(j * P.slice_bytes);
-                    tma_load_2d<kPair>(to, kTwo && kPair && !twice ? &wmap1 : &wmap, (s0 + k + j) * kLinK, v0, bar);
-                    tma_load_2d<kPair>(to + x_at, &xmap, (s0 + k + j) * kLinK, m0, bar);
+                    for (int j = 0; j < kDeep; ++j) {
+                        if (j >= n) break;
+                        const uint32_t to = at + (uint32_t)(j * P.slice_bytes);
+                        tma_load_2d<kPair>(to, kTwo && kPair && !twice ? &wmap1 : &wmap, (s0 + k + j) * kLinK, v0, bar);
+                        tma_load_2d<kPair>(to + x_at, &xmap, (s0 + k + j) * kLinK, m0, bar);
+                    }
                 }
+                __syncwarp();
                 ++issued;
                 if (++stage == P.stages) { stage = 0; phase ^= 1u; }
             }
