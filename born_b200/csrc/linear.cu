@@ -30,16 +30,14 @@ static bool make_map(CUtensorMap* map, const void* p, int rows, int K, int64_t s
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename O, int kCols, bool kPair, bool kTwo>
+template <typename O, int kCols, bool kPair>
 static cudaError_t raise_limit() {
-    return cudaFuncSetAttribute(linear_kernel<O, kCols, kPair, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem);
+    return cudaFuncSetAttribute(linear_kernel<O, kCols, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLinSmem);
 }
 template <typename O>
 static cudaError_t raise_limits() {
-    const cudaError_t e[] = {raise_limit<O, 16, false, false>(), raise_limit<O, 32, false, false>(), raise_limit<O, 64, false, false>(),
-                             raise_limit<O, 128, false, false>(), raise_limit<O, 64, true, false>(), raise_limit<O, 128, true, false>(),
-                             raise_limit<O, 16, false, true>(), raise_limit<O, 32, false, true>(), raise_limit<O, 64, false, true>(),
-                             raise_limit<O, 128, true, true>()};
+    const cudaError_t e[] = {raise_limit<O, 16, false>(), raise_limit<O, 32, false>(), raise_limit<O, 64, false>(),
+                             raise_limit<O, 128, false>(), raise_limit<O, 64, true>(), raise_limit<O, 128, true>()};
     for (const cudaError_t x : e)
         if (x != cudaSuccess) return x;
     return cudaSuccess;
@@ -59,13 +57,13 @@ cudaError_t linear_attrs(LinearLimits& limits) {
         cfg.dynamicSmemBytes = kLinSmem;
         cfg.attrs = &at;
         cfg.numAttrs = 1;
-        e = cudaOccupancyMaxActiveClusters(&limits.clusters[n], linear_kernel<float, 64, false, false>, &cfg);
+        e = cudaOccupancyMaxActiveClusters(&limits.clusters[n], linear_kernel<float, 64, false>, &cfg);
     }
     return e;
 }
 
-template <typename O, int kCols, bool kPair, bool kTwo>
-static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& w1, const CUtensorMap& x, const LinearParams& P, unsigned grid, cudaStream_t st) {
+template <typename O, int kCols, bool kPair>
+static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, unsigned grid, cudaStream_t st) {
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -76,30 +74,25 @@ static cudaError_t launch(const CUtensorMap& w, const CUtensorMap& w1, const CUt
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3(kLinThreads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)P.stages * lin_deep(kTwo) * P.slice_bytes + 1024;
+    cfg.dynamicSmemBytes = (size_t)P.stages * kLinDeep * P.slice_bytes + 1024;
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = kPair || P.splits > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair, kTwo>, w, w1, x, P);
+    return cudaLaunchKernelEx(&cfg, linear_kernel<O, kCols, kPair>, w, x, P);
 }
 template <typename O>
-static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& w1, const CUtensorMap& x, const LinearParams& P, bool pair, bool two, unsigned grid, cudaStream_t st) {
-    if (two) {
-        if (pair) return launch<O, 128, true, true>(w, w1, x, P, grid, st);
-        if (P.cols <= 16) return launch<O, 16, false, true>(w, w1, x, P, grid, st);
-        return P.cols <= 32 ? launch<O, 32, false, true>(w, w1, x, P, grid, st) : launch<O, 64, false, true>(w, w1, x, P, grid, st);
-    }
-    const int cols = P.cols > 16 ? P.cols / 2 : 16;
-    if (pair) return cols <= 64 ? launch<O, 64, true, false>(w, w1, x, P, grid, st) : launch<O, 128, true, false>(w, w1, x, P, grid, st);
-    if (cols <= 16) return launch<O, 16, false, false>(w, w1, x, P, grid, st);
-    if (cols <= 32) return launch<O, 32, false, false>(w, w1, x, P, grid, st);
-    return cols <= 64 ? launch<O, 64, false, false>(w, w1, x, P, grid, st) : launch<O, 128, false, false>(w, w1, x, P, grid, st);
+static cudaError_t launch_as(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& P, bool pair, unsigned grid, cudaStream_t st) {
+    const int cols = P.cols > 16 ? P.cols / 2 : 16;  // of a thread of the epilogue
+    if (pair) return cols <= 64 ? launch<O, 64, true>(w, x, P, grid, st) : launch<O, 128, true>(w, x, P, grid, st);
+    if (cols <= 16) return launch<O, 16, false>(w, x, P, grid, st);
+    if (cols <= 32) return launch<O, 32, false>(w, x, P, grid, st);
+    return cols <= 64 ? launch<O, 64, false>(w, x, P, grid, st) : launch<O, 128, false>(w, x, P, grid, st);
 }
 
 // How a product is cut: the tiles, who shares what, and what that costs.
 struct LinearShape {
-    int cols, m_tiles, v_tiles, doubles, splits, part;
-    bool pair, two;
+    int cols, m_tiles, v_tiles, splits, part;
+    bool pair;
     int64_t cost;  // nanoseconds, about: see below
 };
 // ... with tiles of `most` columns at most
@@ -113,42 +106,27 @@ static LinearShape shape_of(const LinearArgs& A, int most, int num_sms, const Li
     // A pair from 65 columns on: below that the batch's slices are a third of the bytes at most
     S.pair = S.cols > 64 && A.V > kLinRows;
     const int ctas = S.pair ? 2 : 1, unit_rows = ctas * kLinRows, room = num_sms / ctas, x_rows = S.cols / ctas;
-    // Two tiles a CTA for one slice of the batch (up to 128 columns: tensor memory holds two accumulators of both).  For pairs
-    // wherever a CTA has several tiles; where the busiest has an odd number, every CTA's last unit is a single one (one
-    // tile -> two, hidden 4096 and 128256 features: 100 rows 197 -> 188 us, 128 rows 202 -> 193; 8192 x 64000 for 128 rows 213 -> 189).
-    // CTAs on their own read few bytes of the batch and gain nothing (1 row of the first 161 -> 174, 64 rows 175 -> 178; 4096 x
-    // 37000, whose tiles fill their waves to 98%, 51.7 -> 52.5), except where an even number of waves of tiles leaves the GPU
-    // emptier than half as many of two (at 84%: 2048 x 32000 for 1 row 29 -> 25, 64 rows 30.6 -> 28.6; 8192 x 64000 182 -> 165, for 48 rows 192 -> 169).
-    const int singles = (A.V + unit_rows - 1) / unit_rows;
-    int64_t each = ((int64_t)singles * S.m_tiles + room - 1) / room;
-    S.two = S.m_tiles == 1 && each >= 2 && (S.pair ? S.cols <= 128 : S.cols <= 64 && each % 2 == 0 && (int64_t)singles * 10 < each * room * 9);
-    S.v_tiles = singles;
-    S.doubles = 0;
-    if (S.two) {
-        S.doubles = each % 2 ? (int)(each / 2) * room : (singles + 1) / 2;
-        S.v_tiles = S.doubles + (each % 2 ? singles - 2 * S.doubles : 0);
-    }
+    S.v_tiles = (A.V + unit_rows - 1) / unit_rows;
+    const int64_t tiles = (int64_t)S.v_tiles * S.m_tiles, each = (tiles + room - 1) / room;
     // K is shared out while CTAs are left, in parts of four slices at least, over the CTAs of a cluster, and so that all
     // clusters run at once (16 of 8 CTAs do not: 1 x 2048 x 2048 11.3 us with those, 6.8 with 16 of 7).
-    const int64_t tiles = (int64_t)S.v_tiles * S.m_tiles;
     const int slices = (A.K + kLinK - 1) / kLinK;
     int64_t splits = room / tiles;
     if (splits > slices / 4) splits = slices / 4;
     if (splits > kLinMaxCluster / ctas) splits = kLinMaxCluster / ctas;
     while (splits > 1 && limits.clusters[splits * ctas] < tiles) --splits;
-    if (splits < 1 || S.two) splits = 1;
+    if (splits < 1) splits = 1;
     S.part = (int)((slices + splits - 1) / splits);
     S.splits = (slices + S.part - 1) / S.part;
-    // The busiest CTA: 2 ns for 64 elements of a row, of weights or batch; per tile 15 ns a column for the epilogue's end; the
-    // joining of parts 1.5 us and 7 ns a column.  (Fitted to 16 shapes of 80 to 512 rows, within 2 us.)
-    const int64_t reads = S.two ? each / 2 * (2 * kLinRows + x_rows) + each % 2 * (kLinRows + x_rows) : each * (kLinRows + x_rows);
-    S.cost = 2 * S.part * reads + 15 * each * S.cols + (S.splits > 1 ? 1500 + 7 * S.cols : 0);
+    // The busiest CTA: 1.1 ns for 64 elements of a row, of weights or batch; per tile 22 ns a column for the epilogue's end; the
+    // joining of parts 2 us and 25 ns a column.  (Fitted to 16 shapes of 80 to 512 rows, most within 2 us.)
+    S.cost = 11 * S.part * each * (kLinRows + x_rows) / 10 + 22 * each * S.cols + (S.splits > 1 ? 2000 + 25 * S.cols : 0);
     return S;
 }
 
 cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, const LinearLimits& limits, cudaStream_t st) {
     // Wide tiles read the weights once, narrow ones fill the GPU and have less of an end.  Rows x hidden x features with
-    // 256, 128, 64 columns: 256 x 512 x 4096 13.1, 9.8, 6.2 us; 512 x 4096 x 1000 17.2, 15.7, 17.8; 512 x 4096 x 4096 25.9, 29.1, 48.
+    // 256, 128, 64 columns: 256 x 512 x 4096 12.9, 9.2, 4.8 us; 512 x 4096 x 4096 23.7, 18.6, 26.9; 512 x 2048 x 32000 59, 63, 86.
     LinearShape S = shape_of(A, kLinMaxCols, num_sms, limits);
     for (int most = kLinMaxCols / 2; most >= 64 && A.M > 64; most /= 2) {
         const LinearShape o = shape_of(A, most, num_sms, limits);
@@ -157,24 +135,24 @@ cudaError_t linear_launch(const LinearArgs& A, int dtype, int num_sms, const Lin
     LinearParams P;
     memset(&P, 0, sizeof P);
     P.M = A.M; P.K = A.K; P.V = A.V;
-    P.cols = S.cols; P.m_tiles = S.m_tiles; P.v_tiles = S.v_tiles; P.doubles = S.doubles;
+    P.cols = S.cols; P.m_tiles = S.m_tiles; P.v_tiles = S.v_tiles;
     P.splits = S.splits; P.part = S.part;
-    const int w_rows = S.two ? 2 * kLinRows : kLinRows, x_rows = S.pair ? S.cols / 2 : S.cols;
-    P.slice_bytes = (w_rows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
-    P.stages = (kLinSmem - 1024) / (lin_deep(S.two) * P.slice_bytes);
+    const int x_rows = S.pair ? S.cols / 2 : S.cols;
+    P.slice_bytes = (kLinRows + x_rows) * kLinK * 2;  // (8 rows of a slice are 1 KB: atoms stay on 1024 bytes)
+    P.stages = (kLinSmem - 1024) / (kLinDeep * P.slice_bytes);
     if (P.stages > kLinMaxStages) P.stages = kLinMaxStages;
     P.tmem_cols = 32;
-    while (P.tmem_cols < (S.two ? 4 : 2) * P.cols) P.tmem_cols *= 2;
+    while (P.tmem_cols < 2 * P.cols) P.tmem_cols *= 2;
     P.activation = A.activation; P.scale = A.scale; P.inv_scale = 1.0f / A.scale;
     P.bias = A.bias; P.residual = A.residual; P.out = A.out;
     P.residual_stride = A.residual_stride; P.out_stride = A.out_stride;
     P.dev_error = A.dev_error; P.timeout_ns = A.timeout_ns;
-    CUtensorMap w, w1, x;
-    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, w_rows) || !make_map(&w1, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
+    CUtensorMap w, x;
+    if (!make_map(&w, A.weight, A.V, A.K, A.weight_stride, kLinRows) || !make_map(&x, A.x, A.M, A.K, A.x_stride, x_rows)) return cudaErrorInvalidValue;
     const int64_t units = (int64_t)P.v_tiles * P.m_tiles * P.splits, room = S.pair ? num_sms / 2 : num_sms;
     const unsigned grid = (unsigned)(units < room ? units : room) * (S.pair ? 2u : 1u);
-    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, w1, x, P, S.pair, S.two, grid, st);
-    return launch_as<__nv_bfloat16>(w, w1, x, P, S.pair, S.two, grid, st);
+    if (dtype == BORN_DTYPE_F32) return launch_as<float>(w, x, P, S.pair, grid, st);
+    return launch_as<__nv_bfloat16>(w, x, P, S.pair, grid, st);
 }
 
 }  // namespace born

@@ -12,10 +12,6 @@
 // for every 128 rows of weights, and 256 columns of it twice the weights' bytes: out of L2, 256 rows of hidden
 // 4096 over 128256 features took 330 us with that.
 //
-// Up to 128 columns a CTA takes two such tiles at a time (kTwo) where the launch finds that it pays, 256 v for one
-// slice of the batch: L2 hands out some 8.5 TB/s in all, and the batch's slices count as much as the weights there.  128
-// rows of hidden 4096, 128256 features take 193 us, 202 without (its bytes 171).
-//
 // The tensor core cuts partial sums off rather than rounding them, once per 16 products, which adds up: 4.3e-6 of
 // the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded.
 //
@@ -43,7 +39,7 @@ constexpr int kLinK = 64;          // elements of a slice: 128 bytes, one swizzl
 constexpr int kLinChunk = 8;       // slices that the tensor core sums
 constexpr int kLinMaxCols = 256;   // m of a tile
 constexpr int kLinMaxStages = 12;
-__host__ __device__ constexpr int lin_deep(bool two) { return two ? 1 : 2; }  // slices of a ring stage
+constexpr int kLinDeep = 2;        // slices of a ring stage
 constexpr int kLinThreads = 384;   // warps: 0 TMA, 1 products, 2 tensor memory, 3 idle, 4..11 epilogue
 constexpr int kLinSmem = 220 * 1024;
 
@@ -51,7 +47,6 @@ struct LinearParams {
     int M, K, V;
     int cols;          // m of a tile
     int v_tiles, m_tiles;
-    int doubles;       // pairs in kTwo: so many units have two tiles a CTA, those behind them one
     int splits, part;  // CTAs (pairs) of a tile; slices of each
     int stages, slice_bytes, tmem_cols;  // of a CTA
     int activation;
@@ -211,11 +206,10 @@ __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // kCols: columns of the tile that a thread of the epilogue holds at most (the two groups of four warps take half
-// of the tile's columns each, or the first one all 16; in kTwo a tile each).
-template <typename O, int kCols, bool kPair, bool kTwo>
+// of the tile's columns each, or the first one all 16).
+template <typename O, int kCols, bool kPair>
 __global__ void __launch_bounds__(kLinThreads, 1)
-linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wmap1, const __grid_constant__ CUtensorMap xmap,
-              const __grid_constant__ LinearParams P) {
+linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ LinearParams P) {
     extern __shared__ uint8_t raw[];
     __shared__ LinearShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (known to be uniform)
@@ -226,16 +220,10 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     const int first = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int units = P.v_tiles * P.m_tiles * P.splits;      // tiles, times the parts of K
     const int all_slices = (P.K + kLinK - 1) / kLinK;
-    const int groups = kTwo || P.cols > 16 ? 2 : 1;          // of warps that take part in the epilogue
-    constexpr int kMine = kTwo ? 2 * kLinRows : kLinRows;    // v of this CTA
-    constexpr int kTileRows = kPair ? 2 * kMine : kMine;     // v of a unit
-    constexpr int kDeep = lin_deep(kTwo);
-    const int stage_bytes = kDeep * P.slice_bytes;
-    const auto is_double = [&](int u) { return kTwo && (!kPair || u < P.doubles); };
-    const auto first_v = [&](int u, int t) {  // of the unit in this CTA
-        if (!kTwo) return t / P.m_tiles * kTileRows + rank * kMine;
-        return is_double(u) ? u * kTileRows + rank * kMine : P.doubles * kTileRows + (u - P.doubles) * (kTileRows / 2) + rank * kLinRows;
-    };
+    const int groups = P.cols > 16 ? 2 : 1;          // of warps that take part in the epilogue
+    constexpr int kTileRows = kPair ? 2 * kLinRows : kLinRows;  // v of a unit
+    const int stage_bytes = kLinDeep * P.slice_bytes;
+    const auto first_v = [&](int t) { return t / P.m_tiles * kTileRows + rank * kLinRows; };  // of a tile in this CTA
     if (tid == 0) {
         for (int i = 0; i < P.stages; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -263,8 +251,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     if constexpr (kPair) cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sh.tmem;
-    const uint32_t x_at = kMine * kLinK * 2;  // the batch's slice behind the weights' one
-    const int acc_cols = kTwo ? 2 * P.cols : P.cols;
+    const uint32_t x_at = kLinRows * kLinK * 2;  // the batch's slice behind the weights' one
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -277,25 +264,23 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         bool ok = true;
         for (int u = first; u < units && ok; u += step) {
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
-            const int v0 = first_v(u, t);
-            const bool twice = is_double(u);
-            const int bytes = P.slice_bytes - (kTwo && !twice ? kLinRows * kLinK * 2 : 0);
+            const int v0 = first_v(t);
             const int m0 = t % P.m_tiles * P.cols + (kPair ? rank * (P.cols / 2) : 0);
-            for (int k = 0; k < slices; k += kDeep) {
+            for (int k = 0; k < slices; k += kLinDeep) {
                 if (!__all_sync(0xffffffffu, lin_wait(sh, &sh.empty[stage], phase ^ 1u, P.timeout_ns))) {
                     ok = false;
                     break;
                 }
                 const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * stage_bytes);
-                const int n = min(kDeep, slices - k);
+                const int n = min(kLinDeep, slices - k);
                 if (issues) {
                     if (rank == 0)
-                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * bytes * (kPair ? 2 : 1)) : "memory");
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * P.slice_bytes * (kPair ? 2 : 1)) : "memory");
 #pragma unroll
-                    for (int j = 0; j < kDeep; ++j) {
+                    for (int j = 0; j < kLinDeep; ++j) {
                         if (j >= n) break;
                         const uint32_t to = at + (uint32_t)(j * P.slice_bytes);
-                        tma_load_2d<kPair>(to, kTwo && kPair && !twice ? &wmap1 : &wmap, (s0 + k + j) * kLinK, v0, bar);
+                        tma_load_2d<kPair>(to, &wmap, (s0 + k + j) * kLinK, v0, bar);
                         tma_load_2d<kPair>(to + x_at, &xmap, (s0 + k + j) * kLinK, m0, bar);
                     }
                 }
@@ -327,9 +312,9 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + (uint32_t)(acc * acc_cols);
+                const uint32_t d = tmem + (uint32_t)(acc * P.cols);
                 const int k1 = min(slices, k0 + kLinChunk);
-                for (int k = k0; k < k1; k += kDeep) {
+                for (int k = k0; k < k1; k += kLinDeep) {
                     if (!__all_sync(0xffffffffu, lin_wait(sh, &sh.full[stage], phase, P.timeout_ns))) {
                         ok = false;
                         break;
@@ -337,17 +322,12 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (issues) {
 #pragma unroll
-                        for (int j = 0; j < kDeep; ++j) {
+                        for (int j = 0; j < kLinDeep; ++j) {
                             if (k + j >= k1) break;
                             const uint32_t at = ring + (uint32_t)(stage * stage_bytes + j * P.slice_bytes);
                             const uint64_t a = smem_desc(at), b = smem_desc(at + x_at);
 #pragma unroll
                             for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d, a + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
-                            if (is_double(u)) {
-                                const uint64_t a2 = smem_desc(at + kLinRows * kLinK * 2);
-#pragma unroll
-                                for (int i = 0; i < kLinK / 16; ++i) mma_bf16<kPair>(d + (uint32_t)P.cols, a2 + 2 * i, b + 2 * i, idesc, (uint32_t)((k + j - k0) | i));
-                            }
                         }
                         mma_commit<kPair>(&sh.empty[stage], pair);
                     }
@@ -364,17 +344,16 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     } else if (warp >= 4 && (warp - 4) >> 2 < groups) {
         // ---- epilogue
         const int group = (warp - 4) >> 2, quad = warp & 3;
-        const int half = kTwo ? P.cols : P.cols / groups, c0 = kTwo ? 0 : group * half;  // its columns
-        const int r0 = (kTwo ? group * kLinRows : 0) + quad * 32 + lane;                 // its v
-        const uint32_t d0 = tmem + ((uint32_t)quad << 21) + (uint32_t)(kTwo ? group * P.cols : c0);
+        const int half = P.cols / groups, c0 = group * half;  // its columns
+        const int r0 = quad * 32 + lane;  // its v
+        const uint32_t d0 = tmem + ((uint32_t)quad << 21) + (uint32_t)c0;
         int n = 0;
         bool ok = true;
         for (int u = first; u < units && ok; u += step) {
             const int t = u / P.splits, s0 = (u - t * P.splits) * P.part, slices = min(P.part, all_slices - s0);
-            const bool idle = kTwo && group && !is_double(u);
-            const int v = first_v(u, t) + r0, m0 = t % P.m_tiles * P.cols + c0;
+            const int v = first_v(t) + r0, m0 = t % P.m_tiles * P.cols + c0;
             const int count = min(half, P.M - m0);  // (none for a group whose columns lie behind the batch)
-            const bool in = v < P.V && !idle;
+            const bool in = v < P.V;
             const float bias = P.bias && in ? P.bias[v] : 0.0f;
             float y[kCols];
             for (int k0 = 0; k0 < slices; k0 += kLinChunk, ++n) {
@@ -386,10 +365,10 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 // (every lane observes the phase itself before it reads what the products wrote)
                 ring_try(smem_u32(&sh.acc_full[acc]), (uint32_t)(n >> 1) & 1u);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = d0 + (uint32_t)(acc * acc_cols);
+                const uint32_t d = d0 + (uint32_t)(acc * P.cols);
 #pragma unroll
                 for (int c = 0; c < kCols; c += 16) {
-                    if (c >= half || idle) break;
+                    if (c >= half) break;
                     uint32_t r[16];
                     tmem_load16(d + (uint32_t)c, r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -408,7 +387,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.acc_empty[acc])) : "memory");
                 }
             }
-            if (!kTwo && P.splits > 1) {  // (every slice has been used up: the sums take the ring's place)
+            if (P.splits > 1) {  // (every slice has been used up: the sums take the ring's place)
                 float* to = sums + c0 * kLinRows + r0;
 #pragma unroll
                 for (int c = 0; c < kCols; ++c)
@@ -416,7 +395,6 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 continue;
             }
             if (!ok) break;
-            if (idle) continue;
             O* out = reinterpret_cast<O*>(P.out) + (int64_t)m0 * P.out_stride + v;
             const O* res = reinterpret_cast<const O*>(P.residual) + (int64_t)m0 * P.residual_stride + v;
             if (P.bias) {
@@ -457,10 +435,10 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
         }
     }
     __syncwarp();
-    if (!kTwo && P.splits > 1) {
+    if (P.splits > 1) {
         // ---- the parts of K: a CTA of the cluster adds up its share of the columns and finishes them
         cluster_sync();
-        const int S = P.splits, t = first / S, row = tid % kLinRows, v = first_v(first, t) + row, m0 = t % P.m_tiles * P.cols;
+        const int S = P.splits, t = first / S, row = tid % kLinRows, v = first_v(t) + row, m0 = t % P.m_tiles * P.cols;
         const int cols = min(P.cols, P.M - m0), stride = kLinThreads / kLinRows * S;
         const float bias = P.bias && v < P.V ? P.bias[v] : 0.0f;
         for (int c = first % S + tid / kLinRows * S; c < cols; c += 4 * stride) {
