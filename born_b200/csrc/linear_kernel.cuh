@@ -2,8 +2,8 @@
 //
 // A decode batch has few rows and a vocabulary many, so the weights take the tile's 128 rows and the
 // batch its columns (16 to 256): D[128 v][n m] = W[128][K] X[n][K]^T, both operands K-major as they lie in
-// memory.  A CTA per SM walks over tiles; a thread fills a ring of 64-element slices of both operands by
-// TMA (128-byte swizzle), a thread issues the tcgen05 products into one of two accumulators in tensor
+// memory.  A CTA per SM walks over tiles; a warp fills a ring of 64-element slices of both operands by
+// TMA (128-byte swizzle), a warp issues the tcgen05 products into one of two accumulators in tensor
 // memory, eight warps empty the other one: a lane holds one v, so that a column of 32 lanes is a
 // contiguous piece of an output row.
 //
@@ -18,10 +18,15 @@
 // Where the tiles are too few for the GPU, the CTAs (or pairs) of a cluster share one, each with a part of K (splits).  They
 // leave their sums in the place of their rings; every CTA adds up a share of the columns out of all of them, in the
 // order of the parts, and finishes those.  8192 x 1024 weights for one row: 45 us on the eight SMs that have a tile, 15
-// with the sums in scratch and the last CTA adding them up, 9.8 so.
+// with the sums in scratch and the last CTA adding them up, 6.8 so.
 //
-// What bounds it: the bytes of the weights for few rows (1 row of the above: 161 us, the bytes' floor), then what L2 hands
-// out of weights and batch together (64 rows 175 us); 256 rows 244 us, 160 of them the tensor pipe's.
+// One thread's instructions set the pace wherever the slices are small: wait, fence, four products, arrival took 600 cycles
+// a slice, whatever its bytes.  So a ring stage has two slices (256 x 8192 x 2000 24 -> 20.5 us), and the warps that load and that
+// issue products stay together with one elected lane (-> 17.8): their loops run on the uniform side.
+//
+// What bounds it, hidden 4096, 128256 features: the bytes of the weights for few rows (1 row 158 us, 64 rows 167, of 161 and
+// 166), then what L2 hands out of weights and batch together (128 rows 180, of 171); 256 rows 224 to 234 us, 181 of
+// bytes and 160 of products, with the GPU's clock near its power limit.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>

@@ -24,8 +24,8 @@
  *     CUDA/NCCL codes to the latter.
  *
  * Ownership: the caller owns every input and output buffer.  The library owns only its
- * workspace.  What the sampling kernel needs (segment records, mass blocks, tickets), what a beam
- * step leaves between its CTAs (records, tickets) and born_linear's partial sums (9.7 MB) are
+ * workspace.  What the sampling kernel needs (segment records, mass blocks, tickets) and what a
+ * beam step leaves between its CTAs (records, tickets; born_linear needs none) are
  * allocated in born_sampler_create and never per call.  Three kinds of scratch are grown to
  * the largest request seen instead, because their size depends on the call: the staging
  * mirrors of BORN_MEM_HOST calls, the aligned fp32 copy that whole-vocabulary rows need when
