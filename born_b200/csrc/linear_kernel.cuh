@@ -88,11 +88,10 @@ __device__ __forceinline__ bool lin_wait(LinearShared& sh, uint64_t* bar, uint32
     sh.failed = 1;
     return false;
 }
-// Bounded wait whatever happened elsewhere.
-__device__ __forceinline__ void lin_settle(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
-    const unsigned long long t0 = global_timer_ns();
+// Waits for a phase until `until` (a time) at most, whatever happened elsewhere.
+__device__ __forceinline__ void lin_settle(uint32_t bar, uint32_t parity, unsigned long long until) {
     for (uint32_t it = 0; it < kMbarSpinLimit && !ring_try(bar, parity); ++it)
-        if ((it & 15u) == 15u && global_timer_ns() - t0 > limit_ns) break;
+        if ((it & 15u) == 15u && global_timer_ns() > until) break;
 }
 
 __device__ __forceinline__ bool elected() {
@@ -294,13 +293,18 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 if (++stage == P.stages) { stage = 0; phase ^= 1u; }
             }
         }
-        // the copies in flight land before the CTA ends (bounded, whatever happened to the others; the first CTA's
-        // barriers count the second one's too, and neither ends before the other)
-        const int last = rank != 0 ? 0 : issued < P.stages ? (int)issued : P.stages;
-        for (int i = 0; i < last; ++i) {
+        // What is on its way into this CTA arrives before the CTA ends (bounded, whatever happened to the others): the
+        // copies, and the products' arrivals, which in a pair come from the other CTA.  The first CTA's barriers count the second
+        // one's copies too, and neither ends before the other; a copy that the second one alone has issued, where the
+        // first one gave up, gets the time of a wait.
+        const unsigned long long until = global_timer_ns() + P.timeout_ns;
+        if (kPair && rank == 0 && !ok) lin_settle(smem_u32(&sh.full[stage]), phase, until);
+        for (int i = issued < P.stages ? (int)issued : P.stages; i > 0; --i) {
             if (--stage < 0) { stage = P.stages - 1; phase ^= 1u; }
-            lin_settle(smem_u32(&sh.full[stage]), phase, P.timeout_ns);
+            if (rank == 0) lin_settle(smem_u32(&sh.full[stage]), phase, until);
+            lin_settle(smem_u32(&sh.empty[stage]), phase, until);
         }
+        if (rank != 0) lin_settle(smem_u32(&sh.drained), 0, until);
     } else if (warp == 1 && rank == 0) {
         // ---- products: D fp32, A and B bf16, both K-major.  The whole warp goes along, one lane issues.
         const bool issues = elected();
@@ -343,9 +347,10 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                 __syncwarp();
             }
         }
-        // tensor memory is given back only after the last product (bounded, like the copies)
+        // tensor memory is given back only after the last product (bounded, like the copies; in a pair either CTA
+        // waits for its own arrival: the second one's load warp does)
         if (issues) mma_commit<kPair>(&sh.drained, pair);
-        lin_settle(smem_u32(&sh.drained), 0, P.timeout_ns);
+        lin_settle(smem_u32(&sh.drained), 0, global_timer_ns() + P.timeout_ns);
     } else if (warp >= 4 && (warp - 4) >> 2 < groups) {
         // ---- epilogue
         const int group = (warp - 4) >> 2, quad = warp & 3;
