@@ -337,14 +337,26 @@ int fill_scan(Handle* h, ScanArgs& A, int B, int G, int V, int dtype, const void
     return BORN_OK;
 }
 
+// Zeroes device memory before it returns.  (On a stream of its own: cudaMemset is asynchronous on the default stream, which
+// nothing orders with the non-blocking streams that calls may be made on, and may have work of others pending.)
+cudaError_t zero_now(void* p, size_t bytes) {
+    cudaStream_t st;
+    cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e != cudaSuccess) return e;
+    e = cudaMemsetAsync(p, 0, bytes, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    const cudaError_t d = cudaStreamDestroy(st);
+    return e != cudaSuccess ? e : d;
+}
+
 int check_device_error(Handle* h) {
     int e = 0;
     CUDA_TRY(h, cudaMemcpy(&e, h->dev_error, sizeof(int), cudaMemcpyDeviceToHost));
     if (e) {
         // tickets of rows that were left unfinished must not leak into the next launch
-        cudaMemset(h->tickets, 0, sizeof(uint32_t) * 2 * (size_t)h->max_rows);
-        if (h->beam_tickets) cudaMemset(h->beam_tickets, 0, sizeof(uint32_t) * (size_t)h->max_batch);
-        cudaMemset(h->dev_error, 0, sizeof(int));
+        CUDA_TRY(h, zero_now(h->tickets, sizeof(uint32_t) * 2 * (size_t)h->max_rows));
+        if (h->beam_tickets) CUDA_TRY(h, zero_now(h->beam_tickets, sizeof(uint32_t) * (size_t)h->max_batch));
+        CUDA_TRY(h, zero_now(h->dev_error, sizeof(int)));
         return fail(h, BORN_ERR_DEVICE_TIMEOUT, "a bounded on-device wait gave up (code %d); outputs of that call are invalid", e);
     }
     return BORN_OK;
@@ -432,9 +444,9 @@ int32_t born_sampler_create(int32_t device, int32_t max_batch, int32_t max_vocab
     h->beam_records_cap = beam_max_records(max_batch, max_vocab, h->num_sms);
     if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->beam_records, (size_t)h->beam_records_cap * sizeof(BeamRecord));
     if (rc == BORN_OK) rc = dev_alloc(h, (void**)&h->beam_tickets, sizeof(uint32_t) * (size_t)max_batch);
-    if (rc == BORN_OK && cudaMemset(h->beam_tickets, 0, sizeof(uint32_t) * (size_t)max_batch) != cudaSuccess) rc = BORN_ERR_CUDA;
-    if (rc == BORN_OK && cudaMemset(h->tickets, 0, sp.tickets) != cudaSuccess) rc = BORN_ERR_CUDA;
-    if (rc == BORN_OK && cudaMemset(h->dev_error, 0, 32 * sizeof(int)) != cudaSuccess) rc = BORN_ERR_CUDA;
+    if (rc == BORN_OK && zero_now(h->beam_tickets, sizeof(uint32_t) * (size_t)max_batch) != cudaSuccess) rc = BORN_ERR_CUDA;
+    if (rc == BORN_OK && zero_now(h->tickets, sp.tickets) != cudaSuccess) rc = BORN_ERR_CUDA;
+    if (rc == BORN_OK && zero_now(h->dev_error, 32 * sizeof(int)) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && scan_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && cluster_limits(h->max_clusters) != cudaSuccess) rc = BORN_ERR_CUDA;
     if (rc == BORN_OK && spec_attrs_all() != cudaSuccess) rc = BORN_ERR_CUDA;
@@ -494,7 +506,7 @@ int64_t born_fallback_rows(void* handle) {
     if (use_device(h)) return -1;
     int n[24];
     if (cudaMemcpy(n, h->dev_error + 1, sizeof n, cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
-    cudaMemset(h->dev_error + 1, 0, sizeof n);
+    if (zero_now(h->dev_error + 1, sizeof n) != cudaSuccess) return -1;
     // by reason: 2 kept-id list of a whole row; more than 1024 candidates for 1 greedy (ties), 5 top-k, 6 min-p;
     // 7 top-p alone: more than 1024 candidates, or a nucleus that reaches below them; 8 a virtual row with
     // more candidates than its selection holds (3 and 4 are not in use)
@@ -783,7 +795,12 @@ int32_t born_history_create(void* handle, int32_t capacity) {
     h->ring = nullptr;
     const size_t words = (size_t)h->max_batch * ((size_t)capacity + 3);
     CUDA_TRY(h, cudaMalloc((void**)&h->ring, words * 4));
-    CUDA_TRY(h, cudaMemset(h->ring, 0, words * 4));
+    const cudaError_t e = zero_now(h->ring, words * 4);
+    if (e != cudaSuccess) {
+        cudaFree(h->ring);
+        h->ring = nullptr;
+    }
+    CUDA_TRY(h, e);
     h->ring_cap = capacity;
     h->workspace += (int64_t)words * 4;
     return BORN_OK;

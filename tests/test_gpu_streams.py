@@ -1,0 +1,45 @@
+"""Calls on streams of their own while the default stream has work pending.
+
+Torch's streams do not wait for the default stream, so nothing that a call on one of them depends on may be left there."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+BUSY = 400_000_000  # clock cycles that the default stream is kept busy for: a fifth of a second and more
+
+
+def busy(stream=None):
+    """Occupies the default stream (or the given one) with a kernel that only waits; returns an event behind it."""
+    import torch
+    with torch.cuda.stream(stream or torch.cuda.default_stream()):
+        torch.cuda._sleep(BUSY)
+        done = torch.cuda.Event()
+        done.record()
+    return done
+
+
+def test_new_handles_and_histories_are_ready(lib):
+    """What a handle and its history start from is there when the calls that make them return."""
+    import torch
+    from born_b200 import Sampler, SamplingConfig
+    B, V, cap = 8, 5000, 40
+    g = torch.Generator(device="cuda").manual_seed(3)
+    z = torch.randn((B, V), generator=g, device="cuda")
+    prompts = torch.randint(0, V, (B, 30), generator=g, device="cuda", dtype=torch.int32)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    end = busy()
+    with Sampler(device=0, max_batch=B, max_vocab=V) as s, torch.cuda.stream(side):
+        s.history_create(cap)
+        s.history_reset(prompts, stream=side.cuda_stream)
+        out = s.sample_next(z, config=SamplingConfig(), stream=side.cuda_stream)
+        beam = s.beam_step(z, torch.zeros(B, device="cuda"), 4, stream=side.cuda_stream)
+        end.synchronize()
+        side.synchronize()
+        tokens, total, _ = s.history_read(B, cap, stream=side.cuda_stream)
+        assert total.tolist() == [31] * B
+        assert np.array_equal(tokens[:, :30], prompts.cpu().numpy())
+        assert torch.equal(out["token"].long(), z.argmax(1)) and np.array_equal(tokens[:, 30], out["token"].cpu().numpy())
+        assert (beam["status"] == 0).all() and (beam["token"] >= 0).all()
+        s.check_error()
