@@ -15,7 +15,7 @@ import ctypes as C
 import math
 from dataclasses import dataclass
 
-from .sampler import BeamConfig, InvalidArgument
+from .sampler import BeamConfig, BeamPool, InvalidArgument
 
 try:
     import torch
@@ -54,12 +54,16 @@ class BeamSearch:
         self.parent_table = torch.empty((self.max_steps, rows), **i32)
         self.scores = torch.empty(rows, dtype=torch.float32, device=dev)
         self.status = torch.empty(rows, **i32)
-        self.pool = sampler.beam_pool(self.groups, self.beams)
+        self.pool = BeamPool(self.groups, self.beams, dev)  # (begin() empties it, on its own stream)
         # (held here: the kernel writes them after the step's call has returned, on whatever stream it was given)
         self.ends = {n: torch.empty((self.groups, self.beams), dtype=d, device=dev) for n, d in
                      (("end_parent", torch.int32), ("end_token", torch.int32), ("end_score", torch.float32))}
         self.logits = torch.empty((rows, self.vocab), dtype=torch.float32, device=dev) if head is not None else None
         self.steps = None
+        # What the tables' memory was last used for is done on this stream at this point; begin() waits for it.
+        self._home = torch.cuda.current_stream(dev)
+        self._made = torch.cuda.Event()
+        self._made.record(self._home)
         if self.history:
             sampler.history_create(self.history)
 
@@ -68,6 +72,9 @@ class BeamSearch:
         histories of all its beams."""
         self.steps = 0
         with self._on(stream):
+            # (a capture may not wait for what is outside it: its replays come behind whatever the caller puts before them)
+            if (stream or 0) != self._home.cuda_stream and not torch.cuda.is_current_stream_capturing():
+                self._made.wait()
             self.scores.fill_(-math.inf)
             self.scores[::self.beams] = 0.0
         self.sampler.beam_pool_reset(self.pool, stream=stream)

@@ -43,3 +43,38 @@ def test_new_handles_and_histories_are_ready(lib):
         assert torch.equal(out["token"].long(), z.argmax(1)) and np.array_equal(tokens[:, 30], out["token"].cpu().numpy())
         assert (beam["status"] == 0).all() and (beam["token"] >= 0).all()
         s.check_error()
+
+
+@pytest.mark.parametrize("history", [0, 24])
+def test_a_search_made_while_the_default_stream_is_busy(lib, history):
+    """A search that is made and run on a side stream while the default stream has work pending finds what it finds alone."""
+    import torch
+    from born_b200 import BeamConfig, BeamSearch, Sampler
+    N, K, V, steps = 3, 4, 700, 8
+    g = torch.Generator(device="cuda").manual_seed(11)
+    z = torch.randn((steps, N * K, V), generator=g, device="cuda") * 2
+    z[:, :, 5] += 5.0  # (hypotheses end in many steps)
+    prompts = torch.randint(0, V, (N, 6), generator=g, device="cuda", dtype=torch.int32)
+    cfg = BeamConfig(stop_tokens=(5,), length_penalty=0.9, presence_penalty=0.5 if history else 0.0)
+
+    def run(s, stream):
+        search = BeamSearch(s, N, K, steps, V, cfg, history=history)
+        search.begin(prompts if history else None, stream=stream)
+        for t in range(steps):
+            search.step(z[t], stream=stream)
+        return search, search.result(stream=stream)
+
+    with Sampler(device=0, max_batch=64, max_vocab=1024) as s:
+        search, alone = run(s, None)
+        torch.cuda.synchronize()
+        assert (search.pool.step >= 0).any()
+        side = torch.cuda.Stream()
+        for current in (torch.cuda.default_stream(), side):
+            end = busy()
+            with torch.cuda.stream(current):
+                search, found = run(s, side.cuda_stream)
+            end.synchronize()
+            torch.cuda.synchronize()
+            for k in alone:
+                assert torch.equal(alone[k], found[k]), k
+        s.check_error()
