@@ -32,6 +32,9 @@ class Head:
     scale: float = 1.0
 
 
+_parked = []  # tables of searches that went while their stream was being captured, which cannot wait for anything
+
+
 class BeamSearch:
     """One search at a time over groups * beams rows of `vocab` tokens, at most max_steps of them.
 
@@ -64,6 +67,7 @@ class BeamSearch:
         self._home = torch.cuda.current_stream(dev)
         self._made = torch.cuda.Event()
         self._made.record(self._home)
+        self._used = None  # event behind the last call on another stream
         if self.history:
             sampler.history_create(self.history)
 
@@ -86,10 +90,32 @@ class BeamSearch:
                 lens = None if lens is None else lens.to(self.scores.device).repeat_interleave(self.beams).contiguous()
             self._prompts = (rows, lens)  # (kept until the copy on the stream has read them)
             self.sampler.history_reset(rows, lens, stream=stream)
+        self._mark(stream)
 
     def _on(self, stream):
         dev = self.scores.device
         return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev))
+
+    def _mark(self, stream):
+        # (the replays of a capture need the search itself)
+        if (stream or 0) != self._home.cuda_stream:
+            with self._on(stream):
+                if not torch.cuda.is_current_stream_capturing():
+                    self._used = self._used or torch.cuda.Event()
+                    self._used.record()
+
+    def __del__(self):
+        """The tables' memory goes back to the stream on which the search was made: that stream waits for the calls on others."""
+        if getattr(self, "_used", None) is None:
+            return
+        try:
+            with torch.cuda.stream(self._home):
+                if torch.cuda.is_current_stream_capturing():
+                    _parked.append(self.__dict__)
+                else:
+                    self._used.wait()
+        except Exception:  # (the interpreter ends, or the device is gone)
+            pass
 
     @property
     def tokens(self):
@@ -121,6 +147,7 @@ class BeamSearch:
         self.steps = t + 1
         for move in moves:
             move.run(stream)
+        self._mark(stream)
         return self.token_table[t]
 
     def result(self, stream=None):
@@ -141,4 +168,5 @@ class BeamSearch:
                     ((p.step, last), (p.parent, self.parent_table[T - 1].view(N, K)), (p.token, self.tokens.view(N, K)))]
             out = {"tokens": torch.empty((N, K, T), **i32), "lens": torch.empty((N, K), **i32)}
         self.sampler.beam_sequences(self.token_table[:T], self.parent_table[:T], *ends, K, out=out, stream=stream)
+        self._mark(stream)
         return {"tokens": out["tokens"], "lens": out["lens"], "scores": scores}

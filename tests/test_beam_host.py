@@ -107,7 +107,7 @@ def test_a_search_starts_on_its_own_stream(fakes, history, current, used):
     at = used or 0
     assert {e[1] for e in log} == {at}
     launches = ["launch"] * (2 if history else 1)
-    assert [e[0] for e in log] == (launches if at == current else ["wait"] + launches)
+    assert [e[0] for e in log if e[0] != "record"] == (launches if at == current else ["wait"] + launches)
 
 
 def test_a_captured_start_waits_for_nothing_outside(fakes):
@@ -118,3 +118,37 @@ def test_a_captured_start_waits_for_nothing_outside(fakes):
     cuda.capturing = True
     search.begin(stream=7)
     assert log == [("launch", 7)]
+
+
+@pytest.mark.parametrize("current,used", [(0, 7), (5, None)])
+def test_a_search_that_goes_leaves_its_memory_behind_its_calls(fakes, current, used):
+    """The tables' memory returns to the stream on which they were made: that stream waits for what was called on another."""
+    from born_b200 import BeamSearch
+    log, cuda, s = fakes(current)
+    search = BeamSearch(s, 2, 4, 5, 100)
+    search.begin(stream=used)
+    assert log[-1] == ("record", used or 0)
+    del search
+    assert log[-1] == ("wait", current)
+
+
+def test_a_search_on_one_stream_needs_no_events(fakes):
+    from born_b200 import BeamSearch
+    log, cuda, s = fakes(7)
+    search = BeamSearch(s, 2, 4, 5, 100)
+    del log[:]
+    search.begin(stream=7)
+    del search
+    assert log == [("launch", 7)]
+
+
+def test_a_search_that_goes_during_a_capture_keeps_its_memory(fakes):
+    from born_b200 import BeamSearch, beam
+    log, cuda, s = fakes(0)
+    search = BeamSearch(s, 2, 4, 5, 100)
+    search.begin(stream=7)
+    table = search.token_table
+    cuda.capturing = True
+    del log[:]
+    del search
+    assert log == [] and beam._parked.pop()["token_table"] is table

@@ -78,3 +78,31 @@ def test_a_search_made_while_the_default_stream_is_busy(lib, history):
             for k in alone:
                 assert torch.equal(alone[k], found[k]), k
         s.check_error()
+
+
+def test_a_search_dropped_before_its_stream_has_run(lib):
+    """The memory of a search that is gone is not handed out while its calls still wait on their stream."""
+    import torch
+    from born_b200 import BeamSearch, Sampler
+    N, K, V, steps = 2, 4, 500, 6
+    z = torch.randn((steps, N * K, V), device="cuda") * 2
+    side = torch.cuda.Stream()
+    with Sampler(device=0, max_batch=64, max_vocab=1024) as s:
+        def run(stream):
+            search = BeamSearch(s, N, K, steps, V)
+            search.begin(stream=stream)
+            for t in range(steps):
+                search.step(z[t], stream=stream)
+            return search.result(stream=stream)
+        alone = run(None)
+        torch.cuda.synchronize()
+        end = busy(side)
+        found = run(side.cuda_stream)
+        # what a program does next with such sizes, on the stream where the search was made
+        next_ones = [torch.full((n,), 7, dtype=torch.int32, device="cuda") for n in (steps * N * K, N * K, N) for _ in range(6)]
+        assert not end.query()
+        torch.cuda.synchronize()
+        for k in alone:
+            assert torch.equal(alone[k], found[k]), k
+        assert all((x == 7).all() for x in next_ones)
+        s.check_error()
