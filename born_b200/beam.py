@@ -160,7 +160,9 @@ class BeamSearch:
         i32 = dict(dtype=torch.int32, device=self.scores.device)
         with self._on(stream):
             going = (p.done == 0)[:, None] & (self.tokens.view(N, K) >= 0)
-            score = torch.where(going, self.scores.view(N, K) / float(T) ** C.c_float(self.config.length_penalty).value, -math.inf)
+            # (as the pool's: in 64 bits, by a division; a Python divisor would be a multiplication by its rounded inverse)
+            norm = torch.full((), float(T) ** C.c_float(self.config.length_penalty).value, dtype=torch.float64, device=self.scores.device)
+            score = torch.where(going, (self.scores.view(N, K).double() / norm).float(), -math.inf)
             scores, order = torch.sort(torch.cat([p.score, score], 1), dim=1, descending=True, stable=True)
             scores, order = scores[:, :K].contiguous(), order[:, :K]
             last = torch.where(going, T - 1, -1).to(torch.int32)
