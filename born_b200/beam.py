@@ -150,6 +150,12 @@ class BeamSearch:
         self._mark(stream)
         return self.token_table[t]
 
+    def _norm(self, length):
+        try:
+            return float(length) ** C.c_float(self.config.length_penalty).value
+        except OverflowError:  # (infinite, as the step's is)
+            return math.inf
+
     def result(self, stream=None):
         """The best `beams` hypotheses of every group, best first: those of the pool and, in groups that are not
         done, the beams that are still going, all by score / length ** length_penalty.  A dict of tokens [groups,
@@ -161,7 +167,7 @@ class BeamSearch:
         with self._on(stream):
             going = (p.done == 0)[:, None] & (self.tokens.view(N, K) >= 0)
             # (as the pool's: in 64 bits, by a division; a Python divisor would be a multiplication by its rounded inverse)
-            norm = torch.full((), float(T) ** C.c_float(self.config.length_penalty).value, dtype=torch.float64, device=self.scores.device)
+            norm = torch.full((), self._norm(T), dtype=torch.float64, device=self.scores.device)
             score = torch.where(going, (self.scores.view(N, K).double() / norm).float(), -math.inf)
             scores, order = torch.sort(torch.cat([p.score, score], 1), dim=1, descending=True, stable=True)
             scores, order = scores[:, :K].contiguous(), order[:, :K]

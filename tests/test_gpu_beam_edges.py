@@ -31,3 +31,17 @@ def test_beams_that_go_on_are_normalised_as_the_pool(s):
         norm = np.float64(3) ** np.float64(np.float32(penalty))
         want = (search.scores.cpu().numpy().astype(np.float64) / norm).astype(np.float32).reshape(N, K)
         assert np.array_equal(got, -np.sort(-want, axis=1))
+
+
+def test_length_penalties_beyond_all_numbers(s):
+    """length^length_penalty is infinite: every score is (negative) zero, the beams keep their order."""
+    import torch
+    from born_b200 import BeamConfig, BeamSearch
+    N, K, V = 2, 4, 100
+    search = BeamSearch(s, N, K, 4, V, BeamConfig(length_penalty=600.0))
+    search.begin()
+    for t in range(4):
+        search.step(torch.randn((N * K, V), device="cuda"))
+    found = search.result()
+    assert (found["scores"] == 0).all() and (found["lens"] == 4).all()
+    assert torch.equal(found["tokens"][:, :, 3], search.tokens.view(N, K))
