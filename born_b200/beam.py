@@ -74,6 +74,8 @@ class BeamSearch:
     def begin(self, prompts=None, lens=None, stream=None):
         """Start a search: one empty beam per group.  prompts [groups, n] (int32) with optional lens fill the
         histories of all its beams."""
+        if self.history and prompts is not None:
+            self._check_prompts(prompts, lens)
         self.steps = 0
         with self._on(stream):
             # (a capture may not wait for what is outside it: its replays come behind whatever the caller puts before them)
@@ -91,6 +93,13 @@ class BeamSearch:
             self._prompts = (rows, lens)  # (kept until the copy on the stream has read them)
             self.sampler.history_reset(rows, lens, stream=stream)
         self._mark(stream)
+
+    def _check_prompts(self, prompts, lens):
+        # (their elements are read as they lie in memory)
+        if prompts.ndim != 2 or int(prompts.shape[0]) != self.groups or prompts.dtype != torch.int32:
+            raise InvalidArgument(f"prompts must be [{self.groups}, n] int32, not {tuple(prompts.shape)} {prompts.dtype}")
+        if lens is not None and (tuple(lens.shape) != (self.groups,) or lens.dtype != torch.int32):
+            raise InvalidArgument(f"lens must be [{self.groups}] int32, not {tuple(lens.shape)} {lens.dtype}")
 
     def _on(self, stream):
         dev = self.scores.device

@@ -152,3 +152,18 @@ def test_a_search_that_goes_during_a_capture_keeps_its_memory(fakes):
     del log[:]
     del search
     assert log == [] and beam._parked.pop()["token_table"] is table
+
+
+def test_prompts_of_another_type_or_shape_are_refused(fakes):
+    from born_b200 import BeamSearch, InvalidArgument
+    log, cuda, s = fakes(0)
+    search = BeamSearch(s, 3, 2, 5, 100, history=8)
+    good, lens = torch.arange(12, dtype=torch.int32).view(3, 4), torch.tensor([4, 0, 2], dtype=torch.int32)
+    for prompts, n in ((good.long(), None), (good.float(), None), (good[:2], None), (good.view(6, 2), None), (good[0], None),
+                       (good, lens.long()), (good, lens[:2]), (good, lens[:, None])):
+        with pytest.raises(InvalidArgument):
+            search.begin(prompts, n)
+        assert search.steps is None
+    search.begin(good, lens)
+    rows, n = s.loaded
+    assert torch.equal(rows, good.repeat_interleave(2, 0)) and n.tolist() == [4, 4, 0, 0, 2, 2]
