@@ -121,7 +121,7 @@ __device__ __forceinline__ double pow2_down(int k) { return k < -1000 ? 0.0 : __
 // off by ex2's 2^-22 and by 2^-25 of the fraction, however far z is from the maximum, which a scaled difference
 // from the maximum would not give.  Sums of 32 in 32 bits, beyond that in 64.  z0 is 0 but for logits so large
 // that the whole numbers would not fit: those are taken relative to the maximum (what is near it is then exact,
-// and only that counts).
+// and only that counts).  All logits here are times BeamArgs::z_scale.
 struct BeamSum {
     float c, c_lo;   // log2(e)/T in two parts
     float z0;
@@ -160,8 +160,14 @@ struct BeamSum {
         asm("mad.lo.u32 %0, %1, 0xff800000, %2;" : "=r"(o) : "r"(__float_as_uint(r)), "r"(__float_as_uint(e)));
         return __uint_as_float(o);
     }
+    // z_scale: of BeamArgs
     template <int N>
-    __device__ __forceinline__ void add(float (&v)[N], float mx) {
+    __device__ __forceinline__ void add(float (&v)[N], float mx, float z_scale) {
+        if (z_scale != 1.0f) {
+            mx *= z_scale;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] *= z_scale;
+        }
         follow(mx);
         if (m == INT_MIN) return;  // (nothing but -inf so far)
         if (z0 != 0.0f) {
@@ -188,6 +194,7 @@ __device__ __forceinline__ double in_units(const BeamArgs& A, double s, int m, f
 }
 // The units for a maximum: 2^m * exp(z0/T) at least as large as exp(mx/T)
 __device__ __forceinline__ void units_of(const BeamArgs& A, float mx, int& m, float& z0) {
+    mx *= A.z_scale;
     const float t = mx * A.scale_log2e;
     const bool large = !(fabsf(t) <= 1048576.0f);
     z0 = large ? mx : 0.0f;
@@ -510,7 +517,7 @@ __device__ __forceinline__ bool merge_row(const BeamArgs& A, int n, int b, bool 
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         // log sum exp((z - m)/T): the units are 2^m1 exp(z1/T)
         const double c = (double)A.scale_log2e + (double)A.scale_lo;
-        offset = (double)score - (log(s) + ((double)m1 - ((double)m - (double)z1) * c) * M_LN2);
+        offset = (double)score - (log(s) + ((double)m1 - ((double)m * (double)A.z_scale - (double)z1) * c) * M_LN2);
     }
     if (lane < K) sh.row_list[b][lane] = kept;
     if (lane < A.n_stop) sh.row_stop[b][lane] = status == BORN_ROW_OK ? stop : -INFINITY;
@@ -879,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                     }
                     __syncwarp();
                     issue_next();
-                    sum.add(v, gm);
+                    sum.add(v, gm, A.z_scale);
                 } else {
                     float v[32];
                     load_half<T, kAligned>(slot, mis, 0, reinterpret_cast<float(&)[16]>(v[0]));
@@ -897,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                     for (int i = 0; i < 4; ++i)
                         mx[i] = max3_nan(max3_nan(max3_nan(v[8 * i], v[8 * i + 1], v[8 * i + 2]), v[8 * i + 3], v[8 * i + 4]), max3_nan(v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]), -INFINITY);
                     gm = max3_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]);
-                    sum.add(v, gm);
+                    sum.add(v, gm, A.z_scale);
                 }
                 if (++sc == slots) { sc = 0; phase ^= 1u; }
                 gkey[at] = (uint16_t)(zkey(gm) >> 16);
@@ -1007,7 +1014,8 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                 for (int i = me; i < G.n_own; i += crew) {
                     const float x = own[g * A.hist_cap + i] >= 0 ? own_z[g * A.hist_cap + i] : -INFINITY;
                     if (!(x > -INFINITY)) continue;
-                    u += __float2ull_rn(one.two(make_float2(x - z1, x - z1)).x * 1099511627776.0f);
+                    const float d = x * A.z_scale - z1;
+                    u += __float2ull_rn(one.two(make_float2(d, d)).x * 1099511627776.0f);
                     add(make_ck(x, own[g * A.hist_cap + i]));
                 }
                 for (int d = 16; d; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d);

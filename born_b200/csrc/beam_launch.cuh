@@ -36,7 +36,11 @@ struct BeamArgs {
     int history_stride;
     uint32_t flags;
     born_row_params params;
-    float temperature, scale_log2e, scale_lo;  // T; log2(e)/T in two parts
+    float temperature;
+    // Of T above 2^100 the inverse has too few bits, at last none, in 32 bits: the logits are scaled by 2^-100 beforehand.  (What
+    // that costs small ones is no part of z/T that counts.)
+    float z_scale;
+    float scale_log2e, scale_lo;  // log2(e)/T/z_scale in two parts
     double inv_T;   // 1/T
     double slack;   // two normalisers in 32 bits are off by less than this together
     int bit_words;  // words of a CTA's bit map

@@ -1151,9 +1151,11 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
     }
     A.flags = a->flags;
     A.temperature = a->params.temperature == 0.0f ? 1.0f : a->params.temperature;
-    A.scale_log2e = (float)(M_LOG2E / (double)A.temperature);
     A.inv_T = 1.0 / (double)A.temperature;
-    A.scale_lo = (float)(M_LOG2E / (double)A.temperature - (double)A.scale_log2e);
+    A.z_scale = A.temperature > 0x1p100f ? 0x1p-100f : 1.0f;
+    const double scale = M_LOG2E / (double)A.temperature / (double)A.z_scale;
+    A.scale_log2e = (float)scale;
+    A.scale_lo = (float)(scale - (double)A.scale_log2e);
     A.scores = a->scores;
     for (int i = 0; i < a->n_stop; ++i) {  // those of the vocabulary, each once
         const int32_t t = a->stop_ids[i];

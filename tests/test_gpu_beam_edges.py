@@ -45,3 +45,68 @@ def test_length_penalties_beyond_all_numbers(s):
     found = search.result()
     assert (found["scores"] == 0).all() and (found["lens"] == 4).all()
     assert torch.equal(found["tokens"][:, :, 3], search.tokens.view(N, K))
+
+
+def dev(x, dtype=None):
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    return t.to(torch.bfloat16) if dtype == "bf16" else t
+
+
+def bits_of(allowed):
+    r, v = allowed.shape
+    pad = np.zeros((r, (v + 31) // 32 * 32), bool)
+    pad[:, :v] = allowed
+    return np.packbits(pad, axis=1, bitorder="little").view(np.uint32).view(np.int32).copy()
+
+
+def normaliser_error(score):
+    """A normaliser is off by at most 11 * 2^-24: an exponential by ex2's 2^-22, 2^-25 of its exponent's fraction and a little
+    for that fraction's second part (half of 2^-24 allows for it and for the 64-bit remainder), a sum of 32 of them by six rounded
+    additions.  The reported score is rounded once."""
+    return 11 * 2.0 ** -24 + np.abs(score) * 2.0 ** -24
+
+
+def check(out, rows, scores, K, T=0.0):
+    """Tokens, parents and statuses as the definition has them, scores within normaliser_error.  rows: fp32 logits, -inf where masked."""
+    got = {k: v.cpu().numpy() for k, v in out.items()}
+    for n in range(len(rows) // K):
+        sl = slice(n * K, (n + 1) * K)
+        want = R.step([r.astype(np.float32) for r in rows[sl]], scores[sl], (), T)
+        for k in ("status", "token", "parent"):
+            assert got[k][sl].tolist() == want[k], (k, n, got[k][sl], want[k])
+        a, b = got["score"][sl].astype(np.float64), np.array(want["score"], dtype=np.float64)
+        assert (np.isinf(a) == np.isinf(b)).all()
+        f = np.isfinite(b)
+        assert (np.abs(a[f] - b[f]) <= normaliser_error(b[f])).all(), (n, (a - b)[f] * 2.0 ** 24)
+
+
+@pytest.mark.parametrize("T", [1e30, 2e30, 4e36, 6e36, 2e37, 1e38, 3.4e38])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("masked", ["mask", "-inf", "history"])
+def test_large_temperatures(s, T, dtype, masked):
+    """Every finite temperature counts a token that is masked or at -inf for nothing, however near the others' weights are."""
+    import torch
+    from born_b200 import BeamConfig
+    rng = np.random.default_rng(int(math.log2(T)))
+    N, K, V = 4, 3, 1500
+    z = (rng.standard_normal((N * K, V)) * np.float32(3e37)).astype(np.float32)
+    if masked != "history":
+        z[::2] = 2.0  # (all weights alike, all tokens equal: z/T of unequal ones would be lost in 64 bits beside the score)
+    if dtype == "bf16":
+        z = torch.from_numpy(z).to(torch.bfloat16).float().numpy()
+    allowed = rng.random((N * K, V)) < 0.4
+    rows = np.where(allowed, z, np.float32(-np.inf))
+    scores = (-20 - 3 * rng.random(N * K)).astype(np.float32)
+    kw, cfg = {}, BeamConfig(temperature=T)
+    if masked == "-inf":
+        z = rows
+    else:
+        kw["mask"] = dev(bits_of(allowed))
+    if masked == "history":
+        pen = dict(presence=2.0)
+        history = rng.integers(0, V, (N * K, 40)).astype(np.int32)
+        rows = np.stack([np.where(allowed[b], R.penalised(z[b], history[b], **pen), np.float32(-np.inf)) for b in range(N * K)])
+        kw["history"], cfg.presence_penalty = dev(history), 2.0
+    out = s.beam_step(dev(z, dtype), dev(scores), K, config=cfg, **kw)
+    check(out, rows, scores, K, T)
