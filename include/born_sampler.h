@@ -446,7 +446,7 @@ int32_t born_beam_sequences(void* handle, const born_sequences_args* args, void*
 #define BORN_ACT_RELU 1
 #define BORN_ACT_SIGMOID 2
 #define BORN_ACT_TANH 3 /* scale * tanh(y / scale): caps logits at +-scale */
-#define BORN_ACT_GELU 4 /* 0.5 y (1 + erf(y / sqrt 2)) */
+#define BORN_ACT_GELU 4 /* 0.5 y erfc(-y / sqrt 2) */
 #define BORN_ACT_SILU 5
 
 typedef struct born_linear_args {

@@ -1,5 +1,4 @@
 """The output head where its parts meet: launches on one another's heels."""
-import numpy as np  # noqa: F401
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +40,30 @@ def test_launches_that_overlap(s, shapes):
             wrong += (call.out != want).sum()
     s.check_error()
     assert int(wrong) == 0
+
+
+def test_gelu_far_below_zero(s):
+    """0.5 y erfc(-y/sqrt 2) to a relative bound: 1/sqrt 2 and its product with y are rounded (2 * 2^-24), which erfc enlarges by
+    y^2 + 1 at most (t erfc'(t)/erfc(t) <= 2t^2 + 1), erfcf is within 4 ulp (8 * 2^-24), the product and the result round once each;
+    below 2^-126 the same ulps are 2^-149."""
+    import torch
+    V = 30000
+    y = torch.linspace(-14.0, 14.0, V, device="cuda")
+    x, w = torch.zeros((2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((V, 64), dtype=torch.bfloat16, device="cuda")
+    got = s.linear(x, w, bias=y, activation="gelu").double()
+    d = y.double()
+    want = 0.5 * d * torch.special.erfc(-d / 2 ** 0.5)
+    most = want.abs() * 2.0 ** -24 * (2 * (d * d + 1) + 10) + (4 * d.abs() + 2) * 2.0 ** -149
+    assert ((got - want).abs() <= most).all()
+    low = s.linear(x, w, bias=y, activation="gelu", out_dtype=torch.bfloat16).double()
+    assert ((low - want).abs() <= most + want.abs() * 2.0 ** -8 + 2.0 ** -134).all()
+
+
+def test_gelu_of_what_is_no_number(s):
+    import torch
+    y = torch.tensor([float("inf"), float("nan"), float("-inf"), 0.0, 1e30, -1e30, 3e38, -3e38, -30.0, 30.0], device="cuda")
+    x, w = torch.zeros((1, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((len(y), 64), dtype=torch.bfloat16, device="cuda")
+    got = s.linear(x, w, bias=y, activation="gelu")[0].tolist()
+    assert got[0] == float("inf") and got[1] != got[1] and got[2] != got[2]  # (the formula's -inf * 0)
+    f32 = torch.tensor([0.0, 1e30, 0.0, 3e38, 0.0, 0.0, 30.0], device="cuda").tolist()
+    assert got[3:] == f32
