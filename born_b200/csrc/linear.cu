@@ -98,11 +98,7 @@ struct LinearShape {
 // ... with tiles of `most` columns at most
 static LinearShape shape_of(const LinearArgs& A, int most, int num_sms, const LinearLimits& limits) {
     LinearShape S;
-    // as few column tiles as hold the rows, of equal widths
-    S.m_tiles = (A.M + most - 1) / most;
-    const int unit = A.M <= 16 ? 16 : 32;  // (a multiple of 16 for either half of the epilogue)
-    S.cols = ((A.M + S.m_tiles - 1) / S.m_tiles + unit - 1) / unit * unit;
-    S.m_tiles = (A.M + S.cols - 1) / S.cols;
+    linear_columns(A.M, most, S.cols, S.m_tiles);
     // A pair from 65 columns on: below that the batch's slices are a third of the bytes at most
     S.pair = S.cols > 64 && A.V > kLinRows;
     const int ctas = S.pair ? 2 : 1, unit_rows = ctas * kLinRows, room = num_sms / ctas, x_rows = S.cols / ctas;

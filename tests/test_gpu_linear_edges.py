@@ -67,3 +67,18 @@ def test_gelu_of_what_is_no_number(s):
     assert got[0] == float("inf") and got[1] != got[1] and got[2] != got[2]  # (the formula's -inf * 0)
     f32 = torch.tensor([0.0, 1e30, 0.0, 3e38, 0.0, 0.0, 30.0], device="cuda").tolist()
     assert got[3:] == f32
+
+
+def test_more_rows_than_a_tiles_width_may_be_added_to(s):
+    """2.14e9 rows of 8, one feature: as many as an int holds beside the tiles' number."""
+    import torch
+    M = 2_140_000_000
+    x = torch.zeros((M, 8), dtype=torch.bfloat16, device="cuda")
+    x[-3:] = whole((3, 8), 1)
+    x[123_456_789] = 1
+    w = whole((1, 8), 2, 1, 4)
+    out = s.linear(x, w)
+    assert torch.equal(out[-3:], (x[-3:].double() @ w.double().t()).float())
+    assert out[123_456_789].item() == w.double().sum().item()
+    assert sum(int((part != 0).sum()) for part in out.split(1 << 28)) <= 4
+    s.check_error()
