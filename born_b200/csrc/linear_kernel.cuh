@@ -107,12 +107,12 @@ __device__ __forceinline__ bool elected() {
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// bar: of the pair's first CTA in kPair, whose bytes both CTAs' copies count towards
+// bar: address in the cluster; in kPair of the pair's first CTA, whose bytes both CTAs' copies count towards
 template <bool kPair>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     if constexpr (kPair)
         asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-                     "l"(map), "r"(x), "r"(y), "r"(bar & 0xFEFFFFFFu)
+                     "l"(map), "r"(x), "r"(y), "r"(bar)
                      : "memory");
     else
         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -168,7 +168,7 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Adds 16 columns of the accumulator to v, or replaces it by them.
+// 16 columns of the accumulator.
 __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -284,6 +284,7 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
     if (warp == 0) {
         // ---- producer: this CTA's rows of weights, its share of the batch's.  (The whole warp, like the products'.)
         const bool issues = elected();
+        const uint32_t counts = kPair ? remote_smem(smem_u32(&sh.full[0]), (int)pair) : smem_u32(&sh.full[0]);
         int stage = 0;
         uint32_t phase = 0;
         long long issued = 0;
@@ -297,11 +298,11 @@ linear_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ 
                     ok = false;
                     break;
                 }
-                const uint32_t bar = smem_u32(&sh.full[stage]), at = ring + (uint32_t)(stage * stage_bytes);
+                const uint32_t bar = counts + (uint32_t)stage * 8u, at = ring + (uint32_t)(stage * stage_bytes);
                 const int n = min(kLinDeep, slices - k);
                 if (issues) {
                     if (rank == 0)
-                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * P.slice_bytes * (kPair ? 2 : 1)) : "memory");
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&sh.full[stage])), "r"(n * P.slice_bytes * (kPair ? 2 : 1)) : "memory");
 #pragma unroll
                     for (int j = 0; j < kLinDeep; ++j) {
                         if (j >= n) break;
