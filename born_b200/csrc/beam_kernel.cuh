@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
         while (ti < t1) {
             const int tok = (pi * A.pb + bi) * kBlkTok;
             const bool there = from && tok < A.V;
-            if (there && lane == 0)
+            if (there && lane == 0 && ti != A.debug_skip_blk)
                 ring_issue(ring0 + (uint32_t)(si * A.slot_bytes), bar0 + (uint32_t)si * 8u, from, tok, min(kBlkTok, A.V - tok), (int)sizeof(T));
             ti += kBeamWarps;
             bi += kBeamWarps;

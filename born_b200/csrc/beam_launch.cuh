@@ -60,6 +60,7 @@ struct BeamArgs {
     uint32_t* tickets;
     int* dev_error;
     unsigned long long timeout_ns;
+    int debug_skip_blk;  // test hook: the copy of this block is never issued (-1: none)
     // device-resident history (born_beam_next)
     int32_t *ring, *ring_total, *ring_len;
     int ring_cap;

@@ -1046,6 +1046,70 @@ int expire_one(Handle* h, const ExpireCase& c, uint8_t* buf, float* host, cudaSt
     }
     return BORN_ERR_DEVICE_TIMEOUT;
 }
+
+// The same of the beam step: groups of two beams, rows of `blocks` blocks, on `sms` SMs.
+struct BeamExpireCase {
+    int groups, blocks, sms, skip;
+    uint32_t failing;  // rows
+};
+constexpr BeamExpireCase kBeamExpireCases[] = {
+    {2, 4, 4, 9, 0x4u},    // a row a CTA: one of the second group's; the other row of the group goes on
+    {2, 12, 1, 13, 0x3u},  // two rows a CTA, which streams them before it records either
+};
+
+int expire_beam(Handle* h, const BeamExpireCase& c, uint8_t* buf, float* host, cudaStream_t st) {
+    const int R = 2 * c.groups, V = c.blocks * kBlkTok;
+    if (h->max_batch < R) return BORN_ERR_DEVICE_TIMEOUT;  // (no tickets for it)
+    const size_t n = (size_t)R * V;
+    int best[8];
+    for (int r = 0; r < R; ++r) {
+        best[r] = 0;
+        for (int t = 0; t < V; ++t) {
+            host[(size_t)r * V + t] = (float)(((uint32_t)r * (uint32_t)V + (uint32_t)t) * 2654435761u >> 8);
+            if (host[(size_t)r * V + t] > host[(size_t)r * V + best[r]]) best[r] = t;
+        }
+    }
+    uint8_t* out = buf + n * 4;  // scores, parents, tokens, new scores, statuses (16 each)
+    CUDA_TRY(h, cudaMemcpyAsync(buf, host, n * 4, cudaMemcpyHostToDevice, st));
+    CUDA_TRY(h, cudaMemsetAsync(out, 0, 5 * 64, st));
+    BeamArgs A;
+    memset(&A, 0, sizeof A);
+    A.N = c.groups; A.K = 2; A.V = V;
+    A.logits = buf; A.row_stride = V;
+    A.temperature = A.z_scale = 1.0f;
+    A.inv_T = 1.0;
+    A.scale_log2e = (float)M_LOG2E;
+    A.scale_lo = (float)(M_LOG2E - (double)A.scale_log2e);
+    A.scores = (const float*)out;
+    A.out_parent = (int32_t*)(out + 64); A.out_token = (int32_t*)(out + 128);
+    A.out_score = (float*)(out + 192); A.out_status = (int32_t*)(out + 256);
+    A.length_norm = 1.0;
+    A.records = h->beam_records;
+    A.tickets = h->beam_tickets;
+    A.dev_error = h->dev_error;
+    A.timeout_ns = 1000000ull;
+    A.debug_skip_blk = c.skip;
+    CUDA_TRY(h, beam_launch(A, BORN_DTYPE_F32, true, c.sms, st));
+    h->launches++;
+    int32_t got[5][16];
+    CUDA_TRY(h, cudaMemcpyAsync(got, out, sizeof got, cudaMemcpyDeviceToHost, st));
+    CUDA_TRY(h, cudaStreamSynchronize(st));
+    int rc;
+    if ((rc = check_device_error(h)) != BORN_ERR_DEVICE_TIMEOUT) return rc;
+    for (int b = 0; b < R; ++b) {
+        const bool fails = (c.failing >> b) & 1u;
+        const int want = fails ? 100 + BORN_ERR_DEVICE_TIMEOUT : BORN_ROW_OK;
+        if (got[4][b] != want)
+            return fail(h, BORN_ERR_CUDA, "expired wait of a beam step, case %d: row %d reports status %d, not %d", (int)(&c - kBeamExpireCases), b, got[4][b], want);
+        // the largest logit of a row is thousands ahead of the next: a row whose group has both goes on once, with that token
+        if (!fails && !((c.failing >> (b ^ 1)) & 1u)) {
+            const int r = got[1][b & ~1] == (b & 1) ? b & ~1 : b | 1;
+            if (got[1][r] != (b & 1) || got[2][r] != best[b])
+                return fail(h, BORN_ERR_CUDA, "expired wait of a beam step, case %d: row %d goes on with another token", (int)(&c - kBeamExpireCases), b);
+        }
+    }
+    return BORN_ERR_DEVICE_TIMEOUT;
+}
 }  // namespace
 
 int32_t born_debug_expire_wait(void* handle, void* stream) {
@@ -1060,6 +1124,8 @@ int32_t born_debug_expire_wait(void* handle, void* stream) {
     rc = BORN_ERR_DEVICE_TIMEOUT;
     for (const ExpireCase& c : kExpireCases)
         if ((rc = expire_one(h, c, (uint8_t*)h->stage[15].p, host, (cudaStream_t)stream)) != BORN_ERR_DEVICE_TIMEOUT) break;
+    for (const BeamExpireCase& c : kBeamExpireCases)
+        if (rc == BORN_ERR_DEVICE_TIMEOUT) rc = expire_beam(h, c, (uint8_t*)h->stage[15].p, host, (cudaStream_t)stream);
     free(host);
     return rc;
 }
@@ -1173,6 +1239,7 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
     A.tickets = h->beam_tickets;
     A.dev_error = h->dev_error;
     A.timeout_ns = h->timeout_ns;
+    A.debug_skip_blk = -1;
     if (ring) {
         A.ring = h->ring;
         A.ring_total = h->ring + (size_t)h->max_batch * h->ring_cap;

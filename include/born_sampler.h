@@ -259,7 +259,7 @@ const char* born_last_error(void* handle);
 const char* born_version(void);
 
 /* Test hook: small launches of every work decomposition (a CTA per row, clusters, slices, ranges, a
- * warp per row) in each of which one bulk copy is withheld and the wait limit is a millisecond, so
+ * warp per row; beam steps of a row and of two rows a CTA) in each of which one bulk copy is withheld and the wait limit is a millisecond, so
  * that the bounded wait gives up.  Returns BORN_ERR_DEVICE_TIMEOUT when every launch reported the
  * expiry, came back and left the right rows failed (the expected outcome), BORN_OK when one did not
  * expire.  The handle stays usable.  Synchronises the stream. */

@@ -110,3 +110,18 @@ def test_large_temperatures(s, T, dtype, masked):
         kw["history"], cfg.presence_penalty = dev(history), 2.0
     out = s.beam_step(dev(z, dtype), dev(scores), K, config=cfg, **kw)
     check(out, rows, scores, K, T)
+
+
+def test_a_wait_that_runs_out(s, lib):
+    """A copy that never comes fails the rows that its CTA had in hand (the hook checks which, and the other groups' tokens) and leaves
+    nothing behind: neither tickets nor an error for the next step."""
+    from born_b200 import _lib as L
+    for _ in range(2):
+        rc = lib.born_debug_expire_wait(s._h, None)
+        assert rc == L.ERR_DEVICE_TIMEOUT, (rc, lib.born_last_error(s._h))
+    for N, K, V in ((3, 5, 1000), (1, 4, 32000), (40, 4, 9000)):
+        rng = np.random.default_rng(V)
+        z = (rng.standard_normal((N * K, V)) * 2).astype(np.float32)
+        scores = (-20 - 3 * rng.random(N * K)).astype(np.float32)
+        check(s.beam_step(dev(z), dev(scores), K), z, scores, K)
+    s.check_error()
