@@ -121,7 +121,7 @@ __device__ __forceinline__ double pow2_down(int k) { return k < -1000 ? 0.0 : __
 // off by ex2's 2^-22 and by 2^-25 of the fraction, however far z is from the maximum, which a scaled difference
 // from the maximum would not give.  Sums of 32 in 32 bits, beyond that in 64.  z0 is 0 but for logits so large
 // that the whole numbers would not fit: those are taken relative to the maximum (what is near it is then exact,
-// and only that counts).  All logits here are times BeamArgs::z_scale.
+// and only that counts).  For temperatures beyond 2^100 it is not defined (BeamArgs::exact).
 struct BeamSum {
     float c, c_lo;   // log2(e)/T in two parts
     float z0;
@@ -160,14 +160,8 @@ struct BeamSum {
         asm("mad.lo.u32 %0, %1, 0xff800000, %2;" : "=r"(o) : "r"(__float_as_uint(r)), "r"(__float_as_uint(e)));
         return __uint_as_float(o);
     }
-    // z_scale: of BeamArgs
     template <int N>
-    __device__ __forceinline__ void add(float (&v)[N], float mx, float z_scale) {
-        if (z_scale != 1.0f) {
-            mx *= z_scale;
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] *= z_scale;
-        }
+    __device__ __forceinline__ void add(float (&v)[N], float mx) {
         follow(mx);
         if (m == INT_MIN) return;  // (nothing but -inf so far)
         if (z0 != 0.0f) {
@@ -194,7 +188,6 @@ __device__ __forceinline__ double in_units(const BeamArgs& A, double s, int m, f
 }
 // The units for a maximum: 2^m * exp(z0/T) at least as large as exp(mx/T)
 __device__ __forceinline__ void units_of(const BeamArgs& A, float mx, int& m, float& z0) {
-    mx *= A.z_scale;
     const float t = mx * A.scale_log2e;
     const bool large = !(fabsf(t) <= 1048576.0f);
     z0 = large ? mx : 0.0f;
@@ -517,12 +510,12 @@ __device__ __forceinline__ bool merge_row(const BeamArgs& A, int n, int b, bool 
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         // log sum exp((z - m)/T): the units are 2^m1 exp(z1/T)
         const double c = (double)A.scale_log2e + (double)A.scale_lo;
-        offset = (double)score - (log(s) + ((double)m1 - ((double)m * (double)A.z_scale - (double)z1) * c) * M_LN2);
+        offset = (double)score - (log(s) + ((double)m1 - ((double)m - (double)z1) * c) * M_LN2);
     }
     if (lane < K) sh.row_list[b][lane] = kept;
     if (lane < A.n_stop) sh.row_stop[b][lane] = status == BORN_ROW_OK ? stop : -INFINITY;
     if (lane == 0) {
-        sh.offset[b] = offset;
+        sh.offset[b] = A.exact ? 0.0 : offset;  // (a number)
         sh.row_max[b] = m;
         sh.status[b] = status;
     }
@@ -571,14 +564,14 @@ __device__ __forceinline__ void finish_group(const BeamArgs& A, int n, BeamShare
         ahead += o > key || (o == key && i < lane);
     }
     const uint32_t who = __ballot_sync(0xffffffffu, key != 0 && ahead == K - 1);
-    double bound = who ? key_value(__shfl_sync(0xffffffffu, key, __ffs(who) - 1)) - A.slack : -INFINITY;
+    double bound = who && !A.exact ? key_value(__shfl_sync(0xffffffffu, key, __ffs(who) - 1)) - A.slack : -INFINITY;
     if (K > 2) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (more[i]) extend_row(A, warp + i * kBeamWarps, bound, sh, heads[i]);
     }
     rank_candidates(A, sh, true, bound);
-    if (const uint32_t refine = sh.refine) {
+    if (const uint32_t refine = A.exact ? ~0u : sh.refine) {
         for (int b = 0; b < K; ++b) {
             if (!((refine >> b) & 1u)) continue;
             const int64_t row = (int64_t)n * K + b;
@@ -694,7 +687,8 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
     const bool hist = kBits && A.history;
     const uint32_t ring0 = smem_u32(dyn) + (uint32_t)(warp * slots * A.slot_bytes), bar0 = smem_u32(bars + warp * slots);
     if (lane == 0)
-        for (int i = 0; i < slots; ++i) mbar_init(bars + warp * slots + i, 1);
+        for (int i = 0; i < slots; ++i)  // (the test hook's waits for an arrival that never comes)
+            mbar_init(bars + warp * slots + i, i + tid == 0 && (int)blockIdx.x == A.debug_stuck_cta ? 2 : 1);
     if (tid == 0) {
         sh.failed = 0;
         mbar_fence_init();
@@ -723,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
         while (ti < t1) {
             const int tok = (pi * A.pb + bi) * kBlkTok;
             const bool there = from && tok < A.V;
-            if (there && lane == 0 && ti != A.debug_skip_blk)
+            if (there && lane == 0)
                 ring_issue(ring0 + (uint32_t)(si * A.slot_bytes), bar0 + (uint32_t)si * 8u, from, tok, min(kBlkTok, A.V - tok), (int)sizeof(T));
             ti += kBeamWarps;
             bi += kBeamWarps;
@@ -886,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                     }
                     __syncwarp();
                     issue_next();
-                    sum.add(v, gm, A.z_scale);
+                    sum.add(v, gm);
                 } else {
                     float v[32];
                     load_half<T, kAligned>(slot, mis, 0, reinterpret_cast<float(&)[16]>(v[0]));
@@ -904,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                     for (int i = 0; i < 4; ++i)
                         mx[i] = max3_nan(max3_nan(max3_nan(v[8 * i], v[8 * i + 1], v[8 * i + 2]), v[8 * i + 3], v[8 * i + 4]), max3_nan(v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]), -INFINITY);
                     gm = max3_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]);
-                    sum.add(v, gm, A.z_scale);
+                    sum.add(v, gm);
                 }
                 if (++sc == slots) { sc = 0; phase ^= 1u; }
                 gkey[at] = (uint16_t)(zkey(gm) >> 16);
@@ -1014,8 +1008,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_kernel(const __grid_constant
                 for (int i = me; i < G.n_own; i += crew) {
                     const float x = own[g * A.hist_cap + i] >= 0 ? own_z[g * A.hist_cap + i] : -INFINITY;
                     if (!(x > -INFINITY)) continue;
-                    const float d = x * A.z_scale - z1;
-                    u += __float2ull_rn(one.two(make_float2(d, d)).x * 1099511627776.0f);
+                    u += __float2ull_rn(one.two(make_float2(x - z1, x - z1)).x * 1099511627776.0f);
                     add(make_ck(x, own[g * A.hist_cap + i]));
                 }
                 for (int d = 16; d; d >>= 1) u += __shfl_xor_sync(0xffffffffu, u, d);

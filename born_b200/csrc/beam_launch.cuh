@@ -37,10 +37,9 @@ struct BeamArgs {
     uint32_t flags;
     born_row_params params;
     float temperature;
-    // Of T above 2^100 the inverse has too few bits, at last none, in 32 bits: the logits are scaled by 2^-100 beforehand.  (What
-    // that costs small ones is no part of z/T that counts.)
-    float z_scale;
-    float scale_log2e, scale_lo;  // log2(e)/T/z_scale in two parts
+    float scale_log2e, scale_lo;  // log2(e)/T in two parts
+    int exact;  // T is above 2^100: at last log2(e)/T is no number of full length in 32 bits, and the bound below which weights count as
+                // 2^-100 overflows (a masked token would make the sum NaN); all normalisers are computed in 64 bits
     double inv_T;   // 1/T
     double slack;   // two normalisers in 32 bits are off by less than this together
     int bit_words;  // words of a CTA's bit map
@@ -60,7 +59,7 @@ struct BeamArgs {
     uint32_t* tickets;
     int* dev_error;
     unsigned long long timeout_ns;
-    int debug_skip_blk;  // test hook: the copy of this block is never issued (-1: none)
+    int debug_stuck_cta;  // test hook: its first warp never sees its first copy land (-1: none)
     // device-resident history (born_beam_next)
     int32_t *ring, *ring_total, *ring_len;
     int ring_cap;

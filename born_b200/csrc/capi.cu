@@ -1049,12 +1049,12 @@ int expire_one(Handle* h, const ExpireCase& c, uint8_t* buf, float* host, cudaSt
 
 // The same of the beam step: groups of two beams, rows of `blocks` blocks, on `sms` SMs.
 struct BeamExpireCase {
-    int groups, blocks, sms, skip;
+    int groups, blocks, sms, stuck;
     uint32_t failing;  // rows
 };
 constexpr BeamExpireCase kBeamExpireCases[] = {
-    {2, 4, 4, 9, 0x4u},    // a row a CTA: one of the second group's; the other row of the group goes on
-    {2, 12, 1, 13, 0x3u},  // two rows a CTA, which streams them before it records either
+    {2, 4, 4, 2, 0x4u},   // a row a CTA: one of the second group's; the other row of the group goes on
+    {2, 12, 1, 0, 0x3u},  // two rows a CTA, which streams them before it records either
 };
 
 int expire_beam(Handle* h, const BeamExpireCase& c, uint8_t* buf, float* host, cudaStream_t st) {
@@ -1076,7 +1076,7 @@ int expire_beam(Handle* h, const BeamExpireCase& c, uint8_t* buf, float* host, c
     memset(&A, 0, sizeof A);
     A.N = c.groups; A.K = 2; A.V = V;
     A.logits = buf; A.row_stride = V;
-    A.temperature = A.z_scale = 1.0f;
+    A.temperature = 1.0f;
     A.inv_T = 1.0;
     A.scale_log2e = (float)M_LOG2E;
     A.scale_lo = (float)(M_LOG2E - (double)A.scale_log2e);
@@ -1088,7 +1088,7 @@ int expire_beam(Handle* h, const BeamExpireCase& c, uint8_t* buf, float* host, c
     A.tickets = h->beam_tickets;
     A.dev_error = h->dev_error;
     A.timeout_ns = 1000000ull;
-    A.debug_skip_blk = c.skip;
+    A.debug_stuck_cta = c.stuck;
     CUDA_TRY(h, beam_launch(A, BORN_DTYPE_F32, true, c.sms, st));
     h->launches++;
     int32_t got[5][16];
@@ -1218,10 +1218,9 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
     A.flags = a->flags;
     A.temperature = a->params.temperature == 0.0f ? 1.0f : a->params.temperature;
     A.inv_T = 1.0 / (double)A.temperature;
-    A.z_scale = A.temperature > 0x1p100f ? 0x1p-100f : 1.0f;
-    const double scale = M_LOG2E / (double)A.temperature / (double)A.z_scale;
-    A.scale_log2e = (float)scale;
-    A.scale_lo = (float)(scale - (double)A.scale_log2e);
+    A.exact = A.temperature > 0x1p100f;
+    A.scale_log2e = (float)(M_LOG2E / (double)A.temperature);
+    A.scale_lo = (float)(M_LOG2E / (double)A.temperature - (double)A.scale_log2e);
     A.scores = a->scores;
     for (int i = 0; i < a->n_stop; ++i) {  // those of the vocabulary, each once
         const int32_t t = a->stop_ids[i];
@@ -1239,7 +1238,7 @@ int beam_run(Handle* h, const born_beam_args* a, bool ring, cudaStream_t st) {
     A.tickets = h->beam_tickets;
     A.dev_error = h->dev_error;
     A.timeout_ns = h->timeout_ns;
-    A.debug_skip_blk = -1;
+    A.debug_stuck_cta = -1;
     if (ring) {
         A.ring = h->ring;
         A.ring_total = h->ring + (size_t)h->max_batch * h->ring_cap;
