@@ -125,3 +125,65 @@ def test_a_wait_that_runs_out(s, lib):
         scores = (-20 - 3 * rng.random(N * K)).astype(np.float32)
         check(s.beam_step(dev(z), dev(scores), K), z, scores, K)
     s.check_error()
+
+
+def lone_scores(s, z, T=0.0, **kw):
+    """Every row a group of one beam at score 0: (reported score, the definition's in 64 bits); -inf logits weigh nothing."""
+    import torch
+    from born_b200 import BeamConfig
+    cfg = BeamConfig(temperature=T, presence_penalty=kw.pop("presence", 0.0))
+    rows = kw.pop("rows", z).double()
+    out = s.beam_step(z, torch.zeros(z.shape[0], device="cuda"), 1, config=cfg, **kw)
+    assert (out["status"] == 0).all()
+    x = (rows - rows.max(1, keepdim=True).values) / float(np.float32(T or 1.0))
+    return out["score"].cpu().numpy().astype(np.float64), -torch.log(torch.exp(x).sum(1)).cpu().numpy()
+
+
+def near(got, want):
+    return (np.abs(got - want) <= normaliser_error(want)).all(), float((np.abs(got - want) * 2.0 ** 24).max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [0.0, 0.37, 1.7, 30.0])
+@pytest.mark.parametrize("V", [1000, 4096, 50001])
+def test_normalisers_of_equal_logits(s, V, T, dtype):
+    """All terms of a row are the same number: whatever its exponential is off by, and its sums' roundings, go one way."""
+    import torch
+    z = (torch.rand((512, 1), generator=torch.Generator(device="cuda").manual_seed(V), device="cuda") * 60 - 30).expand(512, V)
+    z = z.to(torch.bfloat16 if dtype == "bf16" else torch.float32).contiguous()
+    ok, worst = near(*lone_scores(s, z, T))
+    assert ok, worst
+
+
+@pytest.mark.parametrize("border", [72.6817, -72.6817, 70.0, 5000.0])
+@pytest.mark.parametrize("V", [1000, 20000])
+def test_normalisers_at_the_largest_exponents(s, V, border):
+    """|z/T| log2 e just below and above 2^20 (72.68 at T = 1e-4), where the logits begin to be taken relative to the maximum; tokens
+    lie a few steps of fp32 apart, so that all of them weigh."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(V)
+    step = 2.0 ** (math.floor(math.log2(abs(border))) - 23)
+    near_it = border + (torch.randint(-40, 41, (512, 1), generator=g, device="cuda") * 2.0 ** 5 * step)
+    z = (near_it.double() - torch.randint(0, 8, (512, V), generator=g, device="cuda") * step).float()
+    ok, worst = near(*lone_scores(s, z, 1e-4))
+    assert ok, worst
+
+
+def test_normalisers_of_histories(s):
+    """All of a row's mass comes from tokens of the history, and they come in any order."""
+    import torch
+    V = 700
+    g = torch.Generator(device="cuda").manual_seed(9)
+    z = torch.randn((512, V), generator=g, device="cuda")
+    history = torch.stack([torch.randperm(V, generator=g, device="cuda") for _ in range(512)]).to(torch.int32)
+    ok, worst = near(*lone_scores(s, z, 0.0, presence=1.5, history=history, rows=z - 1.5))
+    assert ok, worst
+
+
+@pytest.mark.parametrize("V", [128256, 262144])
+def test_normalisers_of_long_rows(s, V):
+    import torch
+    z = torch.randn((200, V), generator=torch.Generator(device="cuda").manual_seed(V), device="cuda")
+    z[:100] = z[:100].abs() * -0.01  # many terms near the largest
+    ok, worst = near(*lone_scores(s, z))
+    assert ok, worst

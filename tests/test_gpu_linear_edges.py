@@ -82,3 +82,19 @@ def test_more_rows_than_a_tiles_width_may_be_added_to(s):
     assert out[123_456_789].item() == w.double().sum().item()
     assert sum(int((part != 0).sum()) for part in out.split(1 << 28)) <= 4
     s.check_error()
+
+
+@pytest.mark.parametrize("M,K,V", [(1, 4096, 2000), (64, 8192, 1000), (200, 4096, 3000), (256, 8192, 2000)])
+def test_sums_of_512_products(s, M, K, V):
+    """Cut off 32 times at most, before registers add the next ones, rounded.  A partial sum of j steps of 16 has the root mean square
+    sqrt(j/32) of the 512's and is cut off by less than 2^-23 of itself: sum_j sqrt(j/32) 2^-23 = 21.8 * 2^-23 of the result if all go
+    one way.  The additions round by half of 2^-23 of their partial sums.  (One sum over 4096 products was off by 4.3e-6 = 36 * 2^-23.)"""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(K + M)
+    x = torch.randn((M, K), generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randn((V, K), generator=g, device="cuda").to(torch.bfloat16)
+    want = x.double() @ w.double().t()
+    rms = lambda v: float(v.square().mean().sqrt())  # noqa: E731
+    chunks = K // 512
+    most = sum((j / 32) ** 0.5 for j in range(1, 33)) + 0.5 * sum((i / chunks) ** 0.5 for i in range(1, chunks + 1))
+    assert rms(s.linear(x, w).double() - want) <= most * 2.0 ** -23 * rms(want)
