@@ -1314,8 +1314,10 @@ int32_t born_beam_reorder(void* handle, const born_reorder_args* a, void* stream
     const bool one_row = (int64_t)a->groups * a->beams == 1;
     // the pieces of a row lie apart, and the rows; in either order
     bool apart;
-    if (a->row_stride >= a->plane_stride || a->planes == 1)
-        apart = (a->planes == 1 || a->plane_stride >= piece) && (one_row || a->row_stride >= (a->planes - 1) * (a->planes > 1 ? a->plane_stride : 0) + piece);
+    if (one_row)
+        apart = a->planes == 1 || a->plane_stride >= piece;
+    else if (a->row_stride >= a->plane_stride || a->planes == 1)
+        apart = (a->planes == 1 || a->plane_stride >= piece) && a->row_stride >= (a->planes - 1) * (a->planes > 1 ? a->plane_stride : 0) + piece;
     else
         apart = a->row_stride >= piece && a->plane_stride >= ((int64_t)a->groups * a->beams - 1) * a->row_stride + piece;
     if (!apart) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: rows or pieces overlap (row_stride %lld, plane_stride %lld, piece %lld bytes)",

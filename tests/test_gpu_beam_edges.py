@@ -187,3 +187,25 @@ def test_normalisers_of_long_rows(s, V):
     z[:100] = z[:100].abs() * -0.01  # many terms near the largest
     ok, worst = near(*lone_scores(s, z))
     assert ok, worst
+
+
+def test_the_states_of_a_single_beam(s):
+    """One group of one beam: nothing moves, whatever the layout; pieces that overlap are still refused."""
+    import torch
+    from born_b200 import BeamSearch, InvalidArgument
+    p = torch.zeros(1, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([3], dtype=torch.int32, device="cuda")
+    for shape, dim in (((1, 2, 5, 8), 2), ((1, 5, 2, 8), 1), ((1, 3, 2, 5, 4), 3), ((1, 7), None), ((1,), None)):
+        x = torch.randn(shape, device="cuda")
+        y = x.clone()
+        s.beam_reorder([x], p, 1, lens=None if dim is None else lens, position_dim=dim)
+        assert torch.equal(x, y)
+    call = s.prepare_beam_reorder([torch.randn((1, 2, 5, 8), device="cuda")], p, 1, position_dim=2)
+    call.args.plane_stride -= 4
+    with pytest.raises(InvalidArgument):
+        call.run()
+    cache = torch.randn((1, 2, 5, 8), device="cuda")
+    search = BeamSearch(s, 1, 1, 5, 100)
+    search.begin()
+    search.step(torch.randn((1, 100), device="cuda"), states=[cache], lens=lens, position_dim=2)
+    assert search.tokens.item() >= 0
