@@ -1313,13 +1313,14 @@ int32_t born_beam_reorder(void* handle, const born_reorder_args* a, void* stream
     const int64_t piece = a->positions * a->position_bytes;
     const bool one_row = (int64_t)a->groups * a->beams == 1;
     // the pieces of a row lie apart, and the rows; in either order
+    typedef __int128 wide;  // (a number of strides)
     bool apart;
     if (one_row)
         apart = a->planes == 1 || a->plane_stride >= piece;
     else if (a->row_stride >= a->plane_stride || a->planes == 1)
-        apart = (a->planes == 1 || a->plane_stride >= piece) && a->row_stride >= (a->planes - 1) * (a->planes > 1 ? a->plane_stride : 0) + piece;
+        apart = (a->planes == 1 || a->plane_stride >= piece) && a->row_stride >= (wide)(a->planes - 1) * (a->planes > 1 ? a->plane_stride : 0) + piece;
     else
-        apart = a->row_stride >= piece && a->plane_stride >= ((int64_t)a->groups * a->beams - 1) * a->row_stride + piece;
+        apart = a->row_stride >= piece && a->plane_stride >= ((wide)a->groups * a->beams - 1) * a->row_stride + piece;
     if (!apart) return fail(h, BORN_ERR_INVALID_ARGUMENT, "beam_reorder: rows or pieces overlap (row_stride %lld, plane_stride %lld, piece %lld bytes)",
                             (long long)a->row_stride, (long long)a->plane_stride, (long long)piece);
     if ((int64_t)a->groups * a->n_buffers * a->planes > 0x7fffffff / 4) return fail(h, BORN_ERR_UNSUPPORTED, "beam_reorder: too many pieces for one call");

@@ -209,3 +209,15 @@ def test_the_states_of_a_single_beam(s):
     search.begin()
     search.step(torch.randn((1, 100), device="cuda"), states=[cache], lens=lens, position_dim=2)
     assert search.tokens.item() >= 0
+
+
+def test_strides_whose_multiples_are_beyond_64_bits(s):
+    """Rows and pieces overlap, however the product of a stride and a number of them wraps round."""
+    import torch
+    from born_b200 import InvalidArgument
+    p = torch.zeros(8, dtype=torch.int32, device="cuda")
+    for rows, planes in ((2 ** 61, 2 ** 61), (2 ** 62, 2 ** 61), (2 ** 61, 2 ** 62), (2 ** 61 + 8, 2 ** 62 + 8), (2 ** 62, 2 ** 62 - 64)):
+        call = s.prepare_beam_reorder([torch.zeros((8, 8, 5, 8), device="cuda")], p, 4, position_dim=2)
+        call.args.row_stride, call.args.plane_stride = rows, planes
+        with pytest.raises(InvalidArgument):
+            call.run()
