@@ -221,3 +221,27 @@ def test_strides_whose_multiples_are_beyond_64_bits(s):
         call.args.row_stride, call.args.plane_stride = rows, planes
         with pytest.raises(InvalidArgument):
             call.run()
+
+
+@pytest.mark.parametrize("N,K,V", [(1, 1, 2_000_001), (1, 4, 1_000_000), (1, 16, 700_001), (2, 3, 600_000)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["random", "sorted", "history"])
+def test_rows_of_more_records_than_a_warp_holds(lib, N, K, V, dtype, kind):
+    """A long row is shared by more CTAs than a warp has lanes: the merge goes over their records in several turns."""
+    import torch
+    from born_b200 import BeamConfig, Sampler
+    rng = np.random.default_rng(V + K)
+    z = (rng.standard_normal((N * K, V)) * 2).astype(np.float32)
+    if kind == "sorted":
+        z.sort(axis=1)  # (the best tokens lie together)
+    if dtype == "bf16":
+        z = torch.from_numpy(z).to(torch.bfloat16).float().numpy()
+    scores = (-20 - 3 * rng.random(N * K)).astype(np.float32)
+    kw, rows = {}, z
+    if kind == "history":
+        history = np.argsort(-z, axis=1)[:, :50].astype(np.int32)
+        kw, rows = dict(history=dev(history)), np.stack([R.penalised(z[b], history[b], presence=1.5) for b in range(N * K)])
+    with Sampler(device=0, max_batch=N * K, max_vocab=V) as s:
+        out = s.beam_step(dev(z, dtype), dev(scores), K, config=BeamConfig(presence_penalty=1.5 if kw else 0.0), **kw)
+        check(out, rows, scores, K)
+        s.check_error()
