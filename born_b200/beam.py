@@ -9,7 +9,9 @@ of `Sampler` that make a step, in their order.
     found = search.result()
 
 The reference has no generation at all; its nearest call site is the per-batch loop of
-examples/mnist/main.go:229-245.  Everything stays on the device; nothing synchronises.
+examples/mnist/main.go:229-245.  Everything stays on the device; nothing synchronises but the making of a search
+with a history, which waits until its memory is zeroed.  A search runs on the stream that its calls are given (None: the
+default stream), whichever it was made on; its caller orders calls on different streams.
 """
 import ctypes as C
 import math

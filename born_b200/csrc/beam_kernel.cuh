@@ -14,17 +14,23 @@
 // The normaliser of a row is the only rounded part of that value: tokens of one row order by their
 // logits alone.  It comes from 32-bit exponentials, off by less than A.slack / 2 (beam_slack); where two
 // candidates of different rows are nearer than A.slack and the order matters, the CTA recomputes the
-// normalisers of those rows in 64 bits (row_normaliser), so that the order is that of the definition.
+// normalisers of those rows in 64 bits (row_normaliser), so that the order is that of the definition.  The scores
+// of other rows are reported with the 32-bit normaliser: up to 6e-7 off, 1e-7 as measured, about their own rounding.
 //
-// What bounds it: the bytes of the logits (64 groups of 4 rows of 128256 fp32: 20.1 us of 40.5; the stream ends after
+// What bounds it: the bytes of the logits (64 groups of 4 rows of 128256 fp32: 20.1 us of 41.5; the stream ends after
 // 23) and the chain of round trips behind them, about a microsecond each: bound, groups again, ranking, ticket, records,
 // candidates, which a CTA goes through for its two segments side by side, for two groups that it finishes one after the
-// other.  512 history ids per row cost 10 us: their bits before the stream, their logits and exponentials behind it.
+// other.  Few rows are the chain alone: one group of 4 x 32000 13 us.
+// 512 history ids per row cost 11 us: their bits before the stream, their logits and exponentials behind it.  Repeated
+// ids are counted over the list of all later occurrences, once per id: 1 to 4 us at 512 ids as a text repeats them (156
+// of them), 10 to 15 at 1024 (385).  A pool costs 1.2 to 2.4 us (one thread).  Moving the histories costs 4 to 11 us at
+// 512 ids, 7 to 33 at 1024.
 // bf16 rows are bound by the exponentials, a multiply-add, a conversion and an ex2 per logit: 32 groups of 8 rows of
-// 151936 take 40 us, 12 of them for the bytes.  Few rows are the chain alone: one group of 4 x 32000 12 us.
-// Kept apart by measurement: nothing that the tail reads lives on the stack, for L1 is small beside the
-// rings (closures and lists in local memory: history 64 us instead of 54); two segments side by side rather than
-// one after the other, a team of warps each (42 -> 40.5, history 54 -> 50).
+// 128256 take 40 us, 10 of them for the bytes.  Masked ones (151936, one token in twenty: 47 us of 12.6) wait: with four
+// warps per scheduler 9.3 cycles pass between two instructions of a warp, and the first copies come behind the mask.
+// Kept apart by measurement: none of the tail's lists and closures live on the stack, for L1 is small beside the rings
+// (history 64 us instead of 54); at 128 registers a thread still spills 20 to 90 bytes.  Two segments side by side
+// rather than one after the other, a team of warps each (42 -> 40.5, history 54 -> 50).
 #pragma once
 #include <cuda_runtime.h>
 #include <limits.h>

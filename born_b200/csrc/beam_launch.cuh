@@ -64,7 +64,7 @@ struct BeamArgs {
     int32_t *ring, *ring_total, *ring_len;
     int ring_cap;
 
-    // (blocks < 2^21, grid < 2^10)
+    // (cta <= grid <= 2 SMs, and beam_launch admits 2^32 / (2 SMs) blocks: products fit 32 bits)
     __host__ __device__ int range_start(int cta) const { return (int)((unsigned)cta * (unsigned)blocks / (unsigned)grid); }
     // A segment is a CTA and a piece; from one to the next the CTA or the piece goes up by one, or both, so their
     // sum numbers the segments.  Of the segment that holds block t:
@@ -74,8 +74,7 @@ struct BeamArgs {
 // Records that launches of up to max_batch rows of up to max_vocab tokens leave.
 int64_t beam_max_records(int max_batch, int max_vocab, int num_sms);
 cudaError_t beam_attrs();
-// Fills in how the rows are dealt; cudaErrorInvalidValue where they are too many.
-// cudaErrorNotSupported: more rows than the numbering of the blocks holds
+// Fills in how the rows are dealt and launches; cudaErrorNotSupported: more rows than the numbering of the blocks holds.
 cudaError_t beam_launch(BeamArgs& A, int dtype, bool aligned, int num_sms, cudaStream_t st);
 
 // ---- born_beam_reorder ------------------------------------------------------------------------

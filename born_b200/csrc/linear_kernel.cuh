@@ -13,7 +13,8 @@
 // 4096 over 128256 features took 330 us with that.
 //
 // The tensor core cuts partial sums off rather than rounding them, once per 16 products, which adds up: 4.3e-6 of
-// the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded.
+// the result at K = 4096.  So it sums 512 products at most; those sums are added in registers, rounded: 3.9e-7 there (products and
+// sums in fp32 have 5.9e-7), 4.1e-7 at K = 1000 (2.2e-7).  Shorter sums would keep more and empty the accumulators more often.
 //
 // Where the tiles are too few for the GPU, the CTAs (or pairs) of a cluster share one, each with a part of K (splits).  They
 // leave their sums in the place of their rings; every CTA adds up a share of the columns out of all of them, in the
@@ -25,8 +26,9 @@
 // issue products stay together with one elected lane (-> 17.8): their loops run on the uniform side.
 //
 // What bounds it, hidden 4096, 128256 features: the bytes of the weights for few rows (1 row 158 us, 64 rows 167, of 161 and
-// 166), then what L2 hands out of weights and batch together (128 rows 180, of 171); 256 rows 224 to 234 us, 181 of
-// bytes and 160 of products, with the GPU's clock near its power limit.
+// 166), then what L2 hands out of weights and batch together (128 rows 180, of 171); 256 rows 224 to 229 us after a pause, 181 of
+// bytes and 160 of products.  In a loop of seconds the GPU is at its power limit: 256 rows with tanh 288 to 297 us, 235 to 241 after a
+// pause.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>

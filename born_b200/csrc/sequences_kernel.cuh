@@ -6,9 +6,10 @@
 // steps into 32 chunks each, a half warp per chunk, and compose every chunk's map; a lane per hypothesis walks over all
 // chunks' maps; then all chunks are walked at once, and the tokens are picked and written along the steps.  Longer
 // tables go tile by tile, from the end.
-// Bound by the short pieces that an SM takes in (a group's beams of each row of the tables) and by the walks, some 40
-// cycles a step: 64 groups of 8 beams and 4096 steps take 20.5 us (their bytes 3.9), 47 when every chunk reads its
-// own parents and tokens as it walks, 36 with the parents alone in shared memory, 26 with all of it in one CTA.
+// Bound by a chain of phases: of the 20 us that 64 groups of 8 beams and 4096 steps take (their bytes 3.9) the tables' short
+// pieces (a group's beams of each row) are 5.6, the chunks' maps and their exchange 3.4, the look-up over 128 chunks and the second
+// walk 5.2, the tokens 2.2, start and end 2.4 (clock stamps).  47 us when every chunk reads its own parents and tokens as it
+// walks, 36 with the parents alone in shared memory, 26 with all of it in one CTA.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
