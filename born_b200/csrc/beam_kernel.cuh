@@ -577,7 +577,7 @@ __device__ __forceinline__ void finish_group(const BeamArgs& A, int n, BeamShare
             if (more[i]) extend_row(A, warp + i * kBeamWarps, bound, sh, heads[i]);
     }
     rank_candidates(A, sh, true, bound);
-    if (const uint32_t refine = A.exact ? ~0u : sh.refine) {
+    if (const uint32_t refine = A.exact && !done ? ~0u : sh.refine) {
         for (int b = 0; b < K; ++b) {
             if (!((refine >> b) & 1u)) continue;
             const int64_t row = (int64_t)n * K + b;

@@ -245,3 +245,18 @@ def test_rows_of_more_records_than_a_warp_holds(lib, N, K, V, dtype, kind):
         out = s.beam_step(dev(z, dtype), dev(scores), K, config=BeamConfig(presence_penalty=1.5 if kw else 0.0), **kw)
         check(out, rows, scores, K)
         s.check_error()
+
+
+def test_groups_that_are_done_at_large_temperatures(s):
+    import torch
+    from born_b200 import BeamConfig, _lib as L
+    N, K, V = 3, 4, 900
+    rng = np.random.default_rng(8)
+    z = (rng.standard_normal((N * K, V)) * np.float32(3e37)).astype(np.float32)
+    scores = (-20 - 3 * rng.random(N * K)).astype(np.float32)
+    pool = s.beam_pool(N, K)
+    pool.done[1] = 1
+    out = s.beam_step(dev(z), dev(scores), K, config=BeamConfig(temperature=1e38), pool=pool)
+    assert (out["status"][K:2 * K] == L.ROW_FINISHED).all() and (out["token"][K:2 * K] == -1).all()
+    keep = [r for r in range(N * K) if not K <= r < 2 * K]
+    check({k: v[torch.tensor(keep, device="cuda")] for k, v in out.items()}, z[keep], scores[keep], K, 1e38)
