@@ -328,7 +328,9 @@ int32_t born_mask_wait(void* handle, void* stream);
 
 /* Arguments of born_beam_step.  For every row: penalties and mask as in born_sample, then
  *     s[b][t] = scores[b] + z[t]/T - log sum_j exp(z[j]/T)        (tokens at -inf are no candidates)
- * Candidates of a group are ranked by s in 64 bits, equal ones by b*vocab + t ascending.  The best
+ * Candidates of a group are the `beams` tokens of every row with the largest logits (equal ones by t
+ * ascending) and its stop tokens.  They are ranked by s in 64 bits, equal ones by b*vocab + t ascending
+ * (unequal logits of a row may have equal s where T is very large).  The best
  * `beams` that are no stop tokens go on; stop tokens among the best `beams` of all candidates end.
  * A row whose score is -inf (BORN_ROW_DEAD), or whose status is not BORN_ROW_OK, has no candidates and does not
  * stop the others.  Where fewer than `beams` candidates go on, the remaining rows get parent = the

@@ -260,3 +260,18 @@ def test_groups_that_are_done_at_large_temperatures(s):
     assert (out["status"][K:2 * K] == L.ROW_FINISHED).all() and (out["token"][K:2 * K] == -1).all()
     keep = [r for r in range(N * K) if not K <= r < 2 * K]
     check({k: v[torch.tensor(keep, device="cuda")] for k, v in out.items()}, z[keep], scores[keep], K, 1e38)
+
+
+@pytest.mark.parametrize("T", [1e18, 1e28, 1e34])
+def test_values_that_64_bits_do_not_tell_apart(s, T):
+    """z/T is lost beside the score: all tokens of a row have one value.  The candidates are the row's best by their logits all the same,
+    in the order of their indices."""
+    from born_b200 import BeamConfig
+    N, K, V = 3, 5, 2000
+    rng = np.random.default_rng(4)
+    z = rng.permuted(np.tile(np.arange(V, dtype=np.float32) * 0.01 - 5, (N * K, 1)), axis=1)
+    scores = np.tile(np.float32([-7, -3, -9, -4, -5]), N)  # (of each group the second beam's are ahead of all others')
+    out = {k: v.cpu().numpy() for k, v in s.beam_step(dev(z), dev(scores), K, config=BeamConfig(temperature=T)).items()}
+    for n in range(N):
+        assert out["token"][n * K:(n + 1) * K].tolist() == sorted(np.argsort(-z[n * K + 1])[:K].tolist())
+        assert (out["parent"][n * K:(n + 1) * K] == 1).all()
