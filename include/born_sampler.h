@@ -259,7 +259,8 @@ const char* born_last_error(void* handle);
 const char* born_version(void);
 
 /* Test hook: small launches of every work decomposition (a CTA per row, clusters, slices, ranges, a
- * warp per row; beam steps of a row and of two rows a CTA) in each of which one bulk copy is withheld and the wait limit is a millisecond, so
+ * warp per row; beam steps of a row and of two rows a CTA) in each of which one bulk copy is withheld
+ * (or never seen to land) and the wait limit is a millisecond, so
  * that the bounded wait gives up.  Returns BORN_ERR_DEVICE_TIMEOUT when every launch reported the
  * expiry, came back and left the right rows failed (the expected outcome), BORN_OK when one did not
  * expire.  The handle stays usable.  Synchronises the stream. */
@@ -328,9 +329,9 @@ int32_t born_mask_wait(void* handle, void* stream);
 
 /* Arguments of born_beam_step.  For every row: penalties and mask as in born_sample, then
  *     s[b][t] = scores[b] + z[t]/T - log sum_j exp(z[j]/T)        (tokens at -inf are no candidates)
- * Candidates of a group are the `beams` tokens of every row with the largest logits (equal ones by t
- * ascending) and its stop tokens.  They are ranked by s in 64 bits, equal ones by b*vocab + t ascending
- * (unequal logits of a row may have equal s where T is very large).  The best
+ * Candidates of a group are, of every row, the `beams` tokens with the largest logits that are no stop
+ * tokens (equal ones by t ascending) and the stop tokens.  They are ranked by s in 64 bits, equal ones by
+ * b*vocab + t ascending (unequal logits of a row may have equal s where T is very large).  The best
  * `beams` that are no stop tokens go on; stop tokens among the best `beams` of all candidates end.
  * A row whose score is -inf (BORN_ROW_DEAD), or whose status is not BORN_ROW_OK, has no candidates and does not
  * stop the others.  Where fewer than `beams` candidates go on, the remaining rows get parent = the
