@@ -70,6 +70,7 @@ class BeamSearch:
         self._made = torch.cuda.Event()
         self._made.record(self._home)
         self._used = None  # event behind the last call on another stream
+        self._at = None    # the last call's stream
         if self.history:
             sampler.history_create(self.history)
 
@@ -104,16 +105,19 @@ class BeamSearch:
             raise InvalidArgument(f"lens must be [{self.groups}] int32, not {tuple(lens.shape)} {lens.dtype}")
 
     def _on(self, stream):
-        dev = self.scores.device
-        return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev))
+        return torch.cuda.stream(self._stream(stream))
+
+    def _stream(self, stream):
+        if self._at is None or self._at.cuda_stream != (stream or 0):
+            dev = self.scores.device
+            self._at = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
+        return self._at
 
     def _mark(self, stream):
         # (the replays of a capture need the search itself)
-        if (stream or 0) != self._home.cuda_stream:
-            with self._on(stream):
-                if not torch.cuda.is_current_stream_capturing():
-                    self._used = self._used or torch.cuda.Event()
-                    self._used.record()
+        if (stream or 0) != self._home.cuda_stream and not torch.cuda.is_current_stream_capturing():
+            self._used = self._used or torch.cuda.Event()
+            self._used.record(self._stream(stream))
 
     def __del__(self):
         """The tables' memory goes back to the stream on which the search was made: that stream waits for the calls on others."""
